@@ -65,6 +65,9 @@ def _common_flags() -> list[str]:
         "-fPIC",
         f"--offload-arch={ARCH}",
         "-munsafe-fp-atomics",  # float atomicAdd -> global_atomic_add_f32 (no CAS loop)
+        # no v_pk_{add,mul,fma}_f32: -O3 forms them from scalar float code, and some of their forms
+        # have given wrong results on this machine now and then
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-Wno-unused-result",
         "-DMXDDP_ARCH_GFX950=1",
     ]
