@@ -263,6 +263,38 @@ PYBIND11_MODULE(_C, m) {
                  P<float>(correct), B, C, scale, S(st), loss_scale);
   }, py::arg("logits"), py::arg("y"), py::arg("logp"), py::arg("dlogits"), py::arg("loss_sum"), py::arg("correct"),
      py::arg("B"), py::arg("C"), py::arg("scale"), py::arg("st"), py::arg("loss_scale") = 1.f);
+  m.def("quantize_rows", [](uintptr_t x, int xtype, int64_t ldx, uintptr_t q, int64_t ldq, uintptr_t scale,
+                            int64_t rows, int K, uintptr_t st) {
+    quantize_rows(P<const void>(x), xtype, ldx, P<int8_t>(q), ldq, P<float>(scale), rows, K, S(st));
+  });
+  m.def("linear_int8", [](uintptr_t q, int64_t ldq, uintptr_t xs, uintptr_t w, int64_t ldw, uintptr_t ws,
+                          uintptr_t bias, uintptr_t y, int ytype, int64_t M, int N, int K, bool relu, uintptr_t st) {
+    linear_int8(P<const int8_t>(q), ldq, P<const float>(xs), P<const int8_t>(w), ldw, P<const float>(ws),
+                P<const float>(bias), P<void>(y), ytype, M, N, K, relu, S(st));
+  });
+  m.def("top_logits", [](uintptr_t z, int type, int64_t ldz, int64_t rows, int V, int k, double temperature,
+                         uintptr_t values, uintptr_t index, uintptr_t lse, uintptr_t st) {
+    top_logits(P<const void>(z), type, ldz, rows, V, k, temperature, P<void>(values), P<int32_t>(index),
+               P<float>(lse), S(st));
+  });
+  m.def("distill_fwd", [](uintptr_t z, uintptr_t tv, uintptr_t ti, uintptr_t target, uintptr_t tlse, uintptr_t stats,
+                          int64_t ldz, int64_t rows, int V, int k, int type, int tv_type, bool ti64, bool target64,
+                          double temperature, double hard, uintptr_t loss_rows, uintptr_t loss, bool mean,
+                          uintptr_t st) {
+    distill_fwd(DistillArgs{P<const void>(z), P<const void>(tv), P<const void>(ti), P<const void>(target),
+                            P<const float>(tlse), P<float>(stats), ldz, rows, V, k, type, tv_type, ti64, target64,
+                            temperature, hard},
+                P<float>(loss_rows), P<float>(loss), mean, S(st));
+  });
+  m.def("distill_bwd", [](uintptr_t z, uintptr_t tv, uintptr_t ti, uintptr_t target, uintptr_t tlse, uintptr_t stats,
+                          int64_t ldz, int64_t rows, int V, int k, int type, int tv_type, bool ti64, bool target64,
+                          double temperature, double hard, uintptr_t dloss, bool per_row, uintptr_t dz,
+                          uintptr_t st) {
+    distill_bwd(DistillArgs{P<const void>(z), P<const void>(tv), P<const void>(ti), P<const void>(target),
+                            P<const float>(tlse), P<float>(stats), ldz, rows, V, k, type, tv_type, ti64, target64,
+                            temperature, hard},
+                P<const float>(dloss), per_row, P<void>(dz), S(st));
+  });
   m.def("bn_splits", &bn_splits);
   m.def("bn_fwd_train", [](uintptr_t x, uintptr_t g, uintptr_t b, uintptr_t y, uintptr_t mean, uintptr_t invstd,
                            uintptr_t rm, uintptr_t rv, int N, int C, int HW, float mom, float eps, bool relu,

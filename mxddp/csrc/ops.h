@@ -291,6 +291,40 @@ void synth_templates(float* templates, int C, int D, uint64_t seed, hipStream_t 
 void augment_crop_flip_norm(const float* x, float* y, int N, int C, int H, int W, int pad,
                             const float* mean, const float* std, uint64_t seed, int32_t* counter,
                             hipStream_t st);
+// ---- linear layers in 8-bit integers (int8_linear.hip); element types: lowp.h DType ----
+// |q w| <= 2^14, so up to this many products sum to less than 2^31
+constexpr int kInt8MaxK = (1 << 17) - 1;
+// q [rows][ldq] int8 (columns K .. ldq - 1 zeroed), scale [rows]: x ~ q * scale, scale = max|x| / 127
+// (at least 2^-126; NaN, with q = 0, for a row that is not finite)
+void quantize_rows(const void* x, int xtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K,
+                   hipStream_t st);
+// y [M][N] = relu?((q w^T) xs[m] ws[n] + bias[n])
+void linear_int8(const int8_t* q, int64_t ldq, const float* xs, const int8_t* w, int64_t ldw, const float* ws,
+                 const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu, hipStream_t st);
+
+// ---- learning from a teacher (distill.hip) ----
+constexpr int kTopMax = 256;  // most top logits of a row
+// the k largest logits of each row in falling order (equal ones by index), their indices, and
+// lse = log sum exp(z / temperature)
+void top_logits(const void* z, int type, int64_t ldz, int64_t rows, int V, int k, double temperature, void* values,
+                int32_t* index, float* lse, hipStream_t st);
+struct DistillArgs {
+  const void* z;        // [rows][ldz] student logits
+  const void* tv;       // [rows][k] teacher logits
+  const void* ti;       // [rows][k] their classes (outside [0, V): unused entry)
+  const void* target;   // [rows] or null: the row's class (outside [0, V): row left out)
+  const float* tlse;    // [rows] or null: the teacher's log sum exp(t / T) over all classes
+  float* stats;         // [rows * kDistillStats + 1], written by the forward, read by the backward
+  int64_t ldz, rows;
+  int V, k, type, tv_type, ti64, target64;
+  double temperature, hard;
+};
+constexpr int kDistillStats = 8;
+// loss_rows [rows]: each row's loss; loss (or null): their mean over the counted rows, or their sum
+void distill_fwd(const DistillArgs& a, float* loss_rows, float* loss, bool mean, hipStream_t st);
+// dz [rows][V] = dloss * d loss / dz; dloss: one value, or per_row one for each row's loss
+void distill_bwd(const DistillArgs& a, const float* dloss, bool per_row, void* dz, hipStream_t st);
+
 // argmax(logits)==y counts (metrics)
 void count_correct(const float* logits, const int32_t* y, float* correct, int B, int C, hipStream_t st);
 

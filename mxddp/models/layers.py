@@ -32,6 +32,35 @@ class Linear(nn.Linear):
         return ops.linear(x, self.weight, self.bias, relu=self.fuse_relu)
 
 
+class Int8Linear(nn.Module):
+    """A trained ``Linear`` for answering in 8-bit integers (``ops.linear_int8``): int8 weight with a
+    scale per output channel, inputs quantised per row on the fly, the ReLU in the epilogue.  No
+    parameters and no gradient; ``weight`` rows are padded with zeros to whole 16-byte pieces."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, fuse_relu: bool = False):
+        super().__init__()
+        self.in_features, self.out_features, self.fuse_relu = in_features, out_features, fuse_relu
+        pitch = (in_features + 15) // 16 * 16
+        self.register_buffer("weight", torch.zeros(out_features, pitch, dtype=torch.int8))
+        self.register_buffer("weight_scale", torch.ones(out_features))
+        self.register_buffer("bias", torch.zeros(out_features) if bias else None)
+
+    @classmethod
+    @torch.no_grad()
+    def from_linear(cls, layer: nn.Linear) -> "Int8Linear":
+        new = cls(layer.in_features, layer.out_features, layer.bias is not None, getattr(layer, "fuse_relu", False))
+        new = new.to(layer.weight.device)
+        q, scale = ops.quantize_rows(layer.weight)
+        new.weight[:, :layer.in_features] = q
+        new.weight_scale.copy_(scale)
+        if layer.bias is not None:
+            new.bias.copy_(layer.bias)
+        return new
+
+    def forward(self, x):
+        return ops.linear_int8(x, self.weight[:, :self.in_features], self.weight_scale, self.bias, relu=self.fuse_relu)
+
+
 class ReLU(nn.ReLU):
     def forward(self, x):
         return ops.relu(x)

@@ -23,7 +23,8 @@ from .. import native
 
 __all__ = [
     "conv2d", "linear", "relu", "max_pool2d", "avg_pool2d", "batch_norm", "cross_entropy",
-    "shortcut_pad_add", "stream_of", "refresh_filters", "invalidate_filters",
+    "shortcut_pad_add", "stream_of", "refresh_filters", "invalidate_filters", "quantize_rows", "linear_int8",
+    "top_logits", "TopLogits", "distill_loss",
 ]
 
 
@@ -871,3 +872,8 @@ def set_compute_dtype(dtype: str) -> None:
 
 def compute_dtype() -> str:
     return "bf16" if native().gemm_precision() == 1 else "fp32"
+
+
+# --------------------------------------------------------------------------- 8-bit linear, distillation
+from .distill import TopLogits, distill_loss, top_logits  # noqa: E402
+from .int8 import linear_int8, quantize_rows  # noqa: E402

@@ -1,0 +1,208 @@
+"""Learning from a teacher's top logits (``csrc/distill.hip``), beside ``ops.cross_entropy``.
+
+``top_logits`` keeps what a teacher's answer needs: its k largest logits, their classes, and the
+logarithm of the whole sum of exponentials.  ``distill_loss`` is the student's loss against them,
+with the labels' cross-entropy mixed in where it is asked for; its forward reads the logits once, its
+backward reads them once more and writes their gradient.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import native
+from . import _native, _p, stream_of
+from .lowp import DTYPES, MAX_ROWS, check_device, check_float, on_device, rows_of
+
+MAX_TOP = 256       # csrc/ops.h kTopMax
+MAX_CLASSES = 2**30
+
+
+class TopLogits(NamedTuple):
+    values: torch.Tensor  # [..., k] in falling order, the logits' type
+    index: torch.Tensor   # [..., k] int32 classes
+    lse: torch.Tensor     # [...] float32: log sum exp(logits / temperature)
+
+
+def _check_temperature(t) -> float:
+    t = float(t)
+    if not (t > 0 and math.isfinite(t)):
+        raise ValueError(f"temperature must be a positive number, got {t}")
+    return t
+
+
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    """The k largest logits of each row, in falling order, equal ones by their class.
+
+    ``logits``: [..., V] float32, bfloat16 or float16; 1 <= k <= min(V, 256).  A NaN counts as the
+    largest value.  ``lse`` is taken at ``temperature`` over all classes (infinite or NaN where the
+    largest logit is).  The results carry no gradient."""
+    check_float(logits, "top_logits: logits")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_CLASSES:
+        raise ValueError(f"top_logits: logits must be [..., V] with 1 <= V <= 2^30, got {tuple(logits.shape)}")
+    V = logits.shape[-1]
+    if not 1 <= k <= min(V, MAX_TOP):
+        raise ValueError(f"top_logits: k must be within 1 .. {min(V, MAX_TOP)}, got {k}")
+    temperature = _check_temperature(temperature)
+    logits = logits.detach()
+    if not _native(logits):
+        values, index = torch.sort(logits, dim=-1, descending=True, stable=True)
+        lse = torch.logsumexp(logits.double() / temperature, -1).float()
+        return TopLogits(values[..., :k].contiguous(), index[..., :k].to(torch.int32), lse)
+    z = rows_of(logits)
+    rows = z.shape[0]
+    if rows > MAX_ROWS:
+        raise ValueError(f"top_logits: {rows} rows, at most {MAX_ROWS}")
+    lead = logits.shape[:-1]
+    values = torch.empty((*lead, k), device=z.device, dtype=z.dtype)
+    index = torch.empty((*lead, k), device=z.device, dtype=torch.int32)
+    lse = torch.empty(lead, device=z.device, dtype=torch.float32)
+    with on_device(z):
+        native().top_logits(z.data_ptr(), DTYPES[z.dtype], z.stride(0), rows, V, k, temperature, values.data_ptr(),
+                            index.data_ptr(), lse.data_ptr(), stream_of(z))
+    return TopLogits(values, index, lse)
+
+
+def _args(z, tv, ti, target, tlse, stats, temperature, hard):
+    return (z.data_ptr(), tv.data_ptr(), ti.data_ptr(), _p(target), _p(tlse), stats.data_ptr(), z.stride(0),
+            z.shape[0], z.shape[1], tv.shape[1], DTYPES[z.dtype], DTYPES[tv.dtype], ti.dtype == torch.int64,
+            target is not None and target.dtype == torch.int64, temperature, hard)
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, tv, ti, target, tlse, temperature, hard, reduction):
+        rows = z.shape[0]
+        stats = torch.empty((8 * rows + 1,), device=z.device, dtype=torch.float32)
+        loss_rows = torch.empty((rows,), device=z.device, dtype=torch.float32)
+        loss = torch.empty((), device=z.device, dtype=torch.float32) if reduction != "none" else None
+        with on_device(z):
+            native().distill_fwd(*_args(z, tv, ti, target, tlse, stats, temperature, hard), loss_rows.data_ptr(),
+                                 _p(loss), reduction == "mean", stream_of(z))
+        ctx.save_for_backward(z, tv, ti, target, tlse, stats)
+        ctx.args = (temperature, hard)
+        ctx.per_row = loss is None
+        return loss_rows if loss is None else loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        z, tv, ti, target, tlse, stats = ctx.saved_tensors
+        dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
+        dloss = dloss.to(torch.float32).contiguous()
+        with on_device(z):
+            native().distill_bwd(*_args(z, tv, ti, target, tlse, stats, *ctx.args), dloss.data_ptr(), ctx.per_row,
+                                 dz.data_ptr(), stream_of(z))
+        return dz, None, None, None, None, None, None, None
+
+
+def _distill_rows(z, tv, ti, target, tlse, temperature, hard):
+    """Each row's loss in plain torch (the CPU path), in 64 bits, and which rows count."""
+    V = z.shape[1]
+    used = (ti >= 0) & (ti < V) & (tv != -math.inf)
+    counted = used.any(1) if target is None else (target >= 0) & (target < V)
+    z = torch.where(counted[:, None], z.double(), 0.0)  # what a left-out row holds stays out
+    used = used & counted[:, None]
+    at = torch.where(used, ti, 0).long()
+    zt = z / temperature
+    total = torch.logsumexp(zt, 1)
+    u = torch.where(used, tv.double() / temperature, -math.inf)
+    if tlse is not None:
+        norm = torch.where(counted, tlse.double(), 0.0)
+    else:
+        norm = torch.logsumexp(u, 1)
+        norm = torch.where(used.any(1), norm, 0.0)
+    logp = u - norm[:, None]
+    p = logp.exp()
+    term = torch.where(p != 0, logp, 0.0) - (zt.gather(1, at) - total[:, None])
+    kd = torch.where(p != 0, p * torch.where(p != 0, term, 0.0), 0.0).sum(1)
+    if tlse is not None:
+        named = torch.zeros(z.shape[0], V + 1, dtype=torch.bool, device=z.device)
+        named = named.scatter_(1, torch.where(used, at, V), True)[:, :V]
+        rest = (1 - p.sum(1)).clamp_min(0)
+        has = (rest != 0) & ((zt.detach() > -math.inf) & ~named).any(1)
+        outside = torch.logsumexp(torch.where(named & has[:, None], -math.inf, zt), 1)
+        safe = torch.where(has, rest, 1.0)
+        kd = kd + torch.where(has, safe * (safe.log() - (outside - total)), 0.0)
+    kd = torch.where(used.any(1), kd, 0.0) if tlse is None else kd
+    loss = (1 - hard) * temperature * temperature * kd
+    if hard > 0:
+        y = torch.where(counted, target, 0).long()[:, None]
+        loss = loss + hard * (torch.logsumexp(z, 1) - z.gather(1, y)[:, 0])
+    return torch.where(counted, loss, 0.0), counted
+
+
+def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torch.Tensor,
+                 target: torch.Tensor | None = None, top_lse: torch.Tensor | None = None, temperature: float = 1.0,
+                 hard_weight: float = 0.0, reduction: str = "mean"):
+    """Distillation from a teacher's top logits; with p the teacher's and q = softmax(logits / T)
+
+        loss = (1 - hard_weight) T^2 KL(p || q) + hard_weight cross_entropy(logits, target)
+
+    ``logits``: [..., V], the student's, float32, bfloat16 or float16.  ``top_values`` [..., k] (one
+    of these types) and ``top_index`` [..., k] (int32 or int64): the teacher's logits for k <= 256
+    named classes, as ``top_logits`` gives them.  An entry whose index lies outside [0, V) or whose
+    value is -inf is unused; a class named twice has both entries' share.
+
+    Without ``top_lse`` p is the softmax over the named classes.  With it ([...] float32, the
+    teacher's log sum exp(t / T) at the same temperature) p is the teacher's true probability, and
+    the rest of both distributions, outside the named classes, is compared as one more class (left
+    out where the student gives nothing to the classes outside).
+
+    ``target`` [...] (int32 or int64): the row's class; a row whose target lies outside [0, V) (such
+    as -100) is left out: loss 0, gradient 0, not counted.  Without targets the rows with no used
+    entry are left out.  ``reduction``: "mean" over the counted rows (0 if there are none), "sum", or
+    "none" (each row's loss, [...]).  The loss is float32.  Only ``logits`` get a gradient, once
+    differentiable.
+
+    Both directions may be captured into a graph.  As for every operator, no loss of an earlier eager
+    step may then still hold its autograd graph: torch would draw the stream on which that step met
+    the parameters into the capture, which ends the process."""
+    check_float(logits, "distill_loss: logits", cpu_double=True)
+    check_float(top_values, "distill_loss: top_values", cpu_double=True)
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_CLASSES:
+        raise ValueError(f"distill_loss: logits must be [..., V] with 1 <= V <= 2^30, got {tuple(logits.shape)}")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if top_values.dim() < 1 or top_values.shape[:-1] != lead or top_index.shape != top_values.shape:
+        raise ValueError(f"distill_loss: top_values {tuple(top_values.shape)} and top_index {tuple(top_index.shape)} "
+                         f"must both be {tuple(lead)} + (k,)")
+    k = top_values.shape[-1]
+    if not 1 <= k <= MAX_TOP:
+        raise ValueError(f"distill_loss: k must be within 1 .. {MAX_TOP}, got {k}")
+    for t, name in ((top_index, "top_index"), (target, "target")):
+        if t is not None and t.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"distill_loss: {name} must be int32 or int64, got {t.dtype}")
+    if target is not None and target.shape != lead:
+        raise ValueError(f"distill_loss: target must be {tuple(lead)}, got {tuple(target.shape)}")
+    if top_lse is not None and (top_lse.dtype not in (torch.float32, torch.float64) or top_lse.shape != lead
+                                or (logits.is_cuda and top_lse.dtype != torch.float32)):
+        raise ValueError(f"distill_loss: top_lse must be float32 {tuple(lead)}, got {top_lse.dtype} "
+                         f"{tuple(top_lse.shape)}")
+    for t, name in ((top_values, "top_values"), (top_index, "top_index"), (target, "target"), (top_lse, "top_lse")):
+        check_device(t, logits, name)
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"distill_loss: {name} gets no gradient; detach it")
+    temperature, hard = _check_temperature(temperature), float(hard_weight)
+    if not 0 <= hard <= 1:
+        raise ValueError(f"distill_loss: hard_weight must be within 0 .. 1, got {hard_weight}")
+    if hard > 0 and target is None:
+        raise ValueError("distill_loss: hard_weight needs a target")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"distill_loss: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    z, tv, ti = rows_of(logits), top_values.reshape(-1, k), top_index.reshape(-1, k)
+    target = None if target is None else target.reshape(-1)
+    tlse = None if top_lse is None else top_lse.reshape(-1)
+    if not _native(logits):
+        loss, counted = _distill_rows(z, tv, ti, target, tlse, temperature, hard)
+        loss = loss if logits.dtype == torch.float64 else loss.float()
+        if reduction == "none":
+            return loss.reshape(lead)
+        return loss.sum() / counted.sum().clamp_min(1) if reduction == "mean" else loss.sum()
+    if z.shape[0] > MAX_ROWS:
+        raise ValueError(f"distill_loss: {z.shape[0]} rows, at most {MAX_ROWS}")
+    loss = _DistillLoss.apply(z, tv.contiguous(), ti.contiguous(), None if target is None else target.contiguous(),
+                              None if tlse is None else tlse.contiguous(), temperature, hard, reduction)
+    return loss.reshape(lead) if reduction == "none" else loss

@@ -1,0 +1,110 @@
+"""Linear layers in 8-bit integers (``csrc/int8_linear.hip``), beside ``ops.linear``.
+
+A token (row of x) has one scale, its largest magnitude / 127, and so has each output channel of the
+weight; the product runs on int8 matrix instructions with an exact int32 sum, and the epilogue
+applies both scales, the bias and a ReLU.  Inference only: there is no gradient.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import native
+from .. import ops as _ops
+from . import _native, _p, stream_of
+from .lowp import DTYPES, MAX_ROWS, check_device, check_float, on_device, rows_of
+
+MAX_K = 2**17 - 1  # products of 2^14 each whose sum stays below 2^31
+_TINY = 2.0**-126
+
+
+def quantize_rows(x: torch.Tensor):
+    """``(q, scale)`` with x ~ q * scale[..., None]: int8 rows and one fp32 scale a row.
+
+    ``scale = max|x| / 127`` (at least 2^-126) and ``q = x / scale`` rounded half to even, exactly.
+    A row with an infinity or a NaN has a NaN scale and q = 0.  ``x``: [..., K], float32, bfloat16
+    or float16.  Weights [out, in] give the per-channel scales that ``linear_int8`` takes."""
+    check_float(x, "quantize_rows: x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"quantize_rows: x must be [..., K] with K >= 1, got {tuple(x.shape)}")
+    x = x.detach()
+    if not _native(x):
+        xd = x.double()
+        top = xd.abs().amax(-1)
+        ok = torch.isfinite(top)
+        scale = torch.where(ok, (top / 127).float().clamp_min(_TINY), torch.full_like(top, float("nan")).float())
+        q = torch.where(ok[..., None], (xd / scale.double()[..., None]).round(), torch.zeros_like(xd))
+        return q.to(torch.int8), scale
+    K = x.shape[-1]
+    q = torch.empty(x.shape, device=x.device, dtype=torch.int8)
+    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    _quantize(rows_of(x), q, K, scale)
+    return q, scale
+
+
+def _quantize(x2, q, ldq, scale):
+    if x2.shape[0] > MAX_ROWS:
+        raise ValueError(f"quantize_rows: {x2.shape[0]} rows, at most {MAX_ROWS}")
+    with on_device(x2):
+        native().quantize_rows(x2.data_ptr(), DTYPES[x2.dtype], x2.stride(0), q.data_ptr(), ldq, scale.data_ptr(),
+                               x2.shape[0], x2.shape[1], stream_of(x2))
+
+
+def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
+                relu: bool = False, x_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
+    """``relu?((q @ weight.T) * s[..., None] * weight_scale + bias)`` for (q, s) = quantize_rows(x).
+
+    ``weight``: int8 [N, K], contiguous rows of any stride; ``weight_scale``: float32 [N];
+    ``bias``: float32 [N].  ``x``: [..., K] in float32, bfloat16 or float16, or int8 with its
+    ``x_scale`` [...] (``quantize_rows``: one quantised input for several layers).  The result has
+    ``out_dtype`` (default: x's type, float32 for an int8 x).  K is at most 131071.  No gradient: an
+    ``x`` that requires one is refused while autograd records."""
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear_int8: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    N, K = weight.shape
+    if weight.dtype != torch.int8:
+        raise TypeError(f"linear_int8: weight must be int8, got {weight.dtype}")
+    if not 1 <= K <= MAX_K or N < 1:
+        raise ValueError(f"linear_int8: weight {tuple(weight.shape)}: 1 <= K <= {MAX_K} and N >= 1")
+    given = x.dtype == torch.int8
+    if given:
+        if x_scale is None or x_scale.dtype != torch.float32 or x_scale.shape != x.shape[:-1]:
+            raise ValueError("linear_int8: an int8 x needs its float32 x_scale, one a row")
+    else:
+        check_float(x, "linear_int8: x")
+        if x_scale is not None:
+            raise ValueError("linear_int8: x_scale goes with an int8 x")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad() or detach x")
+    out_dtype = out_dtype or (torch.float32 if given else x.dtype)
+    if out_dtype not in DTYPES:
+        raise TypeError(f"linear_int8: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    for t, name in ((weight_scale, "weight_scale"), (bias, "bias")):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (N,)):
+            raise ValueError(f"linear_int8: {name} must be float32 [{N}], got {t.dtype} {tuple(t.shape)}")
+        check_device(t, x, name)
+    check_device(weight, x, "weight")
+    check_device(x_scale, x, "x_scale")
+    if not _native(x):
+        q, s = (x, x_scale) if given else quantize_rows(x)
+        y = (q.double() @ weight.double().t()) * s.double()[..., None] * weight_scale.detach().double()
+        if bias is not None:
+            y = y + bias.detach().double()
+        return (y.clamp_min(0) if relu else y).to(out_dtype)
+    x2 = rows_of(x.detach())
+    M = x2.shape[0]
+    if M > MAX_ROWS:
+        raise ValueError(f"linear_int8: {M} rows, at most {MAX_ROWS}")
+    weight = weight if weight.stride(1) == 1 or K == 1 else weight.contiguous()
+    y = torch.empty((*x.shape[:-1], N), device=x.device, dtype=out_dtype)
+    if given:
+        q, ldq, s = x2, x2.stride(0), x_scale.contiguous()
+    else:
+        ldq = (K + 15) // 16 * 16
+        q = torch.empty((M, ldq), device=x.device, dtype=torch.int8)
+        s = torch.empty((M,), device=x.device, dtype=torch.float32)
+        _quantize(x2, q, ldq, s)
+    with on_device(x2):
+        native().linear_int8(q.data_ptr(), ldq, s.data_ptr(), weight.data_ptr(), weight.stride(0),
+                             weight_scale.contiguous().data_ptr(), 0 if bias is None else bias.contiguous().data_ptr(),
+                             y.data_ptr(), DTYPES[out_dtype], M, N, K, bool(relu), stream_of(x2))
+    return y

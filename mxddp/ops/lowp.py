@@ -1,0 +1,34 @@
+"""What the operators for fp32, bf16 and fp16 tensors share: their types, rows and checks."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # csrc/lowp.h DType
+MAX_ROWS = 2**31 - 1
+
+
+def check_float(t: torch.Tensor, name: str, cpu_double: bool = False) -> None:
+    if t.dtype not in DTYPES and not (cpu_double and t.dtype == torch.float64 and not t.is_cuda):
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+
+
+def check_device(t: torch.Tensor | None, x: torch.Tensor, name: str) -> None:
+    if t is not None and t.device != x.device:
+        raise ValueError(f"{name} is on {t.device}, the input on {x.device}")
+
+
+def rows_of(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as [rows, last] with contiguous rows (any row stride), copied only where it must be."""
+    n = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(t.numel() // n if n else 0, n)
+    return t if t.stride(1) == 1 or n == 1 else t.contiguous()
+
+
+def on_device(t: torch.Tensor):
+    """Launches go to the current device: make it the tensor's."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)

@@ -1,0 +1,317 @@
+"""8-bit linear layers (ops.quantize_rows, ops.linear_int8, layers.Int8Linear) against the
+definition in 64 bits.
+
+The quantised values have one right answer each (the exact quotient, rounded half to even), so they
+are compared bit for bit.  A product's sum is a whole number; what is left are the roundings of the
+epilogue: the sum to fp32, two scales, the bias, and the result's type, each by half a step.
+"""
+import pytest
+import torch
+
+from mxddp import ops
+from mxddp.models.layers import Int8Linear, Linear
+
+DEVICES = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+E = 2.0**-24
+
+
+def oracle_quantize(x):
+    """q and scale of [M, K] in 64 bits on the CPU; the quotient's rounding by comparison."""
+    x = x.detach().cpu().double()
+    top = x.abs().amax(1)
+    scale = torch.maximum(top / 127, torch.tensor(2.0**-126, dtype=torch.float64)).float()
+    d = x / scale.double()[:, None]
+    low = d.floor()
+    up = (d - low > 0.5) | ((d - low == 0.5) & (low.remainder(2) == 1))
+    return (low + up).to(torch.int8), scale
+
+
+def oracle_linear(q, s, w, ws, bias, relu):
+    prod = (q.cpu().double() @ w.cpu().double().t()) * s.cpu().double()[:, None] * ws.cpu().double()
+    y = prod if bias is None else prod + bias.cpu().double()
+    return (y.clamp_min(0) if relu else y), prod
+
+
+def check_linear(y, q, s, w, ws, bias, relu):
+    want, prod = oracle_linear(q, s, w, ws, bias, relu)
+    # sum to fp32 and two scales: 3 half steps of the product; bias: one of the result
+    b = 0 if bias is None else bias.cpu().double().abs()
+    tol = 3.01 * E * prod.abs() + 1.01 * E * (prod.abs() + b) + torch.finfo(y.dtype).eps / 2 * 1.001 * want.abs()
+    tol = tol + torch.finfo(y.dtype).smallest_normal * torch.finfo(y.dtype).eps  # a subnormal's step
+    far = (y.detach().cpu().double() - want).abs()
+    assert y.shape == want.shape
+    assert bool((far <= tol).all()), f"off by {(far / tol).max().item():.2f} of the bound"
+
+
+def make(M, N, K, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(M, K, generator=g) * torch.exp(torch.randn(K, generator=g))).to(dtype)
+    w = torch.randint(-127, 128, (N, K), generator=g, dtype=torch.int8)
+    ws = torch.rand(N, generator=g) * 0.01 + 1e-4
+    return x, w, ws, torch.randn(N, generator=g)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K", [(1, 1), (3, 7), (5, 64), (2, 1000), (7, 4097), (300, 129), (2, 40000), (1, 131071)])
+def test_quantize_rows(dev, dtype, M, K):
+    x = make(M, 1, K, dtype, M + K)[0]
+    q, s = ops.quantize_rows(x.to(dev))
+    wq, ws = oracle_quantize(x)
+    assert q.dtype == torch.int8 and s.dtype == torch.float32 and q.shape == x.shape and s.shape == (M,)
+    assert torch.equal(s.cpu(), ws) and torch.equal(q.cpu(), wq)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_quantize_rows_halves(dev):
+    """Quotients at and next to a half, either sign: scale 2^e exactly (127 2^e is the maximum)."""
+    for e in (-126, -30, 0, 20):
+        n = torch.arange(-127, 127, dtype=torch.float64)
+        near = torch.stack([n + 0.5, (n + 0.5) * (1 + 2.0**-23), (n + 0.5) * (1 - 2.0**-23)]).reshape(-1)
+        x = torch.cat([near, torch.tensor([127.0], dtype=torch.float64)]).clamp(-127, 127) * 2.0**e
+        x = x.float()[None]
+        q, s = ops.quantize_rows(x.to(dev))
+        wq, ws = oracle_quantize(x)
+        assert torch.equal(s.cpu(), ws) and torch.equal(q.cpu(), wq), e
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_quantize_rows_values(dev):
+    """Rows of zeros, subnormals, the largest numbers, and rows that are not finite."""
+    big = torch.finfo(torch.float32).max
+    x = torch.tensor([[0.0, -0.0, 0.0], [1e-44, -3e-45, 0.0], [big, -big, 1.0], [1.0, float("inf"), 2.0],
+                      [float("nan"), 1.0, 0.0], [1.0, -float("inf"), float("nan")], [2.0, -1.0, 0.5]])
+    q, s = ops.quantize_rows(x.to(dev))
+    q, s = q.cpu(), s.cpu()
+    fine = [0, 1, 2, 6]
+    wq, ws = oracle_quantize(x[fine])
+    assert torch.equal(q[fine], wq) and torch.equal(s[fine], ws)
+    assert torch.isnan(s[[3, 4, 5]]).all() and (q[[3, 4, 5]] == 0).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_quantize_rows_shapes(dev):
+    x = torch.randn(2, 3, 50, generator=torch.Generator().manual_seed(0))
+    want_q, want_s = oracle_quantize(x.reshape(6, 50))
+    wide = torch.zeros(6, 77, device=dev)
+    wide[:, 5:55] = x.reshape(6, 50).to(dev)
+    for v in (x.to(dev), x.to(dev).transpose(0, 1).contiguous().transpose(0, 1),
+              wide[:, 5:55].reshape(2, 3, 50), x.to(dev).permute(2, 0, 1).contiguous().permute(1, 2, 0)):
+        q, s = ops.quantize_rows(v)
+        assert q.shape == (2, 3, 50) and s.shape == (2, 3)
+        assert torch.equal(q.cpu().reshape(6, 50), want_q) and torch.equal(s.cpu().reshape(6), want_s)
+    q, s = ops.quantize_rows(wide[:, 5:55])
+    assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+    q, s = ops.quantize_rows(x[0, 0].to(dev))
+    assert torch.equal(q.cpu(), want_q[0]) and s.shape == () and s.item() == want_s[0].item()
+    q, s = ops.quantize_rows(torch.empty(0, 9, device=dev))
+    assert q.shape == (0, 9) and s.shape == (0,)
+
+
+SIZES = [  # M, N, K: one token and few, rows of 16 bytes or not, tile edges, many tiles
+    (1, 1, 1), (1, 10, 64), (1, 1000, 2048), (1, 4096, 512), (1, 513, 1001), (2, 100, 77), (3, 33, 4096),
+    (8, 640, 256), (15, 257, 100), (16, 256, 1024), (17, 130, 1000), (31, 96, 784), (33, 1000, 1000), (63, 65, 127),
+    (64, 64, 64), (65, 129, 66), (100, 300, 300), (128, 128, 128), (129, 257, 208), (250, 1000, 2048),
+    (256, 256, 256), (257, 255, 1040), (300, 512, 48), (511, 513, 500), (1024, 1000, 16), (1500, 700, 136),
+]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_linear_int8(dev, M, N, K):
+    dtype = TYPES[(M + N) % 3]
+    x, w, ws, b = make(M, N, K, dtype, M * 7 + N)
+    q, s = oracle_quantize(x)
+    args = (x.to(dev), w.to(dev), ws.to(dev))
+    check_linear(ops.linear_int8(*args), q, s, w, ws, None, False)
+    check_linear(ops.linear_int8(*args, b.to(dev), relu=True), q, s, w, ws, b, True)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M,N,K", [(1, 300, 1024), (5, 77, 96), (5, 77, 99), (70, 200, 1000), (300, 300, 512)])
+@pytest.mark.parametrize("out", TYPES)
+def test_linear_int8_given(dev, M, N, K, out):
+    """An int8 input with its scales, all 256 values on both sides (a weight may hold -128)."""
+    g = torch.Generator().manual_seed(K)
+    q = torch.randint(-128, 128, (M, K), generator=g, dtype=torch.int8)
+    w = torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8)
+    s, ws = torch.rand(M, generator=g), torch.rand(N, generator=g) * 1e-3
+    y = ops.linear_int8(q.to(dev), w.to(dev), ws.to(dev), x_scale=s.to(dev), out_dtype=out)
+    assert y.dtype == out
+    check_linear(y, q, s, w, ws, None, False)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M", [1, 20, 200])
+def test_linear_int8_largest_sums(dev, M):
+    """Every product 2^14 over the longest rows: the sum is just below 2^31."""
+    K, N = ops.int8.MAX_K, 20
+    q = torch.full((M, K), -128, dtype=torch.int8, device=dev)
+    w = torch.full((N, K), -128, dtype=torch.int8, device=dev)
+    y = ops.linear_int8(q, w, torch.ones(N, device=dev), x_scale=torch.ones(M, device=dev))
+    assert bool((y.double() == float(torch.tensor(K * 2**14, dtype=torch.float64).float())).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M", [1, 6, 150])
+def test_linear_int8_strides(dev, M):
+    """Rows with other strides and starts: slices of wider tensors, a weight whose rows are padded."""
+    N, K = 140, 112
+    x, w, ws, b = make(M, N, K, torch.bfloat16)
+    q, s = oracle_quantize(x)
+    for off, pad in ((0, 16), (16, 48), (3, 5), (8, 8), (1, 15)):
+        wide = torch.full((N, K + off + pad), 99, dtype=torch.int8, device=dev)
+        wv = wide[:, off:off + K]
+        wv.copy_(w)
+        xw = torch.full((M, K + off + pad), float("nan"), dtype=x.dtype, device=dev)
+        xv = xw[:, off:off + K]
+        xv.copy_(x)
+        check_linear(ops.linear_int8(xv, wv, ws.to(dev), b.to(dev)), q, s, w, ws, b, False)
+        qw = torch.full((M, K + off + pad), 77, dtype=torch.int8, device=dev)
+        qv = qw[:, off:off + K]
+        qv.copy_(q)
+        y = ops.linear_int8(qv, wv, ws.to(dev), b.to(dev), x_scale=s.to(dev))
+        check_linear(y, q, s, w, ws, b, False)
+    # the weight's rows stored column by column; an input of more dimensions; every second scale
+    wt = w.to(dev).t().contiguous().t()
+    ws2 = torch.stack([ws, ws + 1], 1).to(dev)[:, 0]
+    y = ops.linear_int8(x.to(dev)[None, :, None], wt, ws2, b.to(dev))
+    assert y.shape == (1, M, 1, N)
+    check_linear(y[0, :, 0], q, s, w, ws, b, False)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M", [1, 40, 200])
+def test_linear_int8_padded_tail(dev, M):
+    """A weight whose padded rows end with the tensor's own memory, what lies there arbitrary."""
+    N, K = 50, 1001
+    x, w, ws, b = make(M, N, K, torch.float32)
+    q, s = oracle_quantize(x)
+    wide = torch.full((N, 1008), 127, dtype=torch.int8, device=dev)
+    wide[:, :K] = w.to(dev)
+    check_linear(ops.linear_int8(x.to(dev), wide[:, :K], ws.to(dev)), q, s, w, ws, None, False)
+    flat = torch.full((N * 1008 - 7,), 127, dtype=torch.int8, device=dev)  # the last row ends at K
+    view = flat.as_strided((N, K), (1008, 1))
+    view.copy_(w)
+    check_linear(ops.linear_int8(x.to(dev), view, ws.to(dev)), q, s, w, ws, None, False)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_linear_int8_values(dev):
+    """No tokens; a row that is not finite gives NaN there and nowhere else; a ReLU keeps NaN."""
+    x, w, ws, b = make(40, 24, 64, torch.float32)
+    y = ops.linear_int8(x[:0].to(dev), w.to(dev), ws.to(dev))
+    assert y.shape == (0, 24)
+    q, s = oracle_quantize(x)
+    bad = x.clone()
+    bad[3, 5] = float("inf")
+    bad[17, 0] = float("nan")
+    for relu in (False, True):
+        y = ops.linear_int8(bad.to(dev), w.to(dev), ws.to(dev), b.to(dev), relu=relu).cpu()
+        keep = [i for i in range(40) if i not in (3, 17)]
+        assert torch.isnan(y[[3, 17]]).all()
+        check_linear(y[keep], q[keep], s[keep], w, ws, b, relu)
+    # scales whose product leaves fp32's range, with a sum of zero
+    y = ops.linear_int8(torch.zeros(2, 64, dtype=torch.int8, device=dev), w.to(dev), torch.full((24,), 1e30, device=dev),
+                        x_scale=torch.full((2,), 1e30, device=dev))
+    assert (y == 0).all()
+
+
+def test_refusals():
+    x, w, ws, b = make(4, 6, 8, torch.float32)
+    for bad, err in [
+        (lambda: ops.quantize_rows(x.double()), TypeError),
+        (lambda: ops.quantize_rows(torch.tensor(1.0)), ValueError),
+        (lambda: ops.quantize_rows(torch.empty(3, 0)), ValueError),
+        (lambda: ops.linear_int8(x, w.float(), ws), TypeError),
+        (lambda: ops.linear_int8(x.double(), w, ws), TypeError),
+        (lambda: ops.linear_int8(x[:, :7], w, ws), ValueError),
+        (lambda: ops.linear_int8(x, w[0], ws), ValueError),
+        (lambda: ops.linear_int8(x, w, ws[:5]), ValueError),
+        (lambda: ops.linear_int8(x, w, ws.double()), ValueError),
+        (lambda: ops.linear_int8(x, w, ws, b.half()), ValueError),
+        (lambda: ops.linear_int8(x, w, ws, b[:, None]), ValueError),
+        (lambda: ops.linear_int8(x, w, ws, x_scale=torch.ones(4)), ValueError),
+        (lambda: ops.linear_int8(x.to(torch.int8), w, ws), ValueError),
+        (lambda: ops.linear_int8(x.to(torch.int8), w, ws, x_scale=torch.ones(3)), ValueError),
+        (lambda: ops.linear_int8(x.to(torch.int8), w, ws, x_scale=torch.ones(4).double()), ValueError),
+        (lambda: ops.linear_int8(x, w, ws, out_dtype=torch.int8), TypeError),
+        (lambda: ops.linear_int8(x.clone().requires_grad_(), w, ws), RuntimeError),
+        (lambda: ops.linear_int8(torch.zeros(1, 2**17), torch.zeros(2, 2**17, dtype=torch.int8), ws[:2]), ValueError),
+        (lambda: ops.linear_int8(x, w, ws.to("meta")), ValueError),
+    ]:
+        with pytest.raises(err):
+            bad()
+    with torch.no_grad():
+        ops.linear_int8(x.clone().requires_grad_(), w, ws)
+
+
+@pytest.mark.gpu
+def test_refusals_native(cuda):
+    """The native entries refuse sizes that their kernels do not take."""
+    from mxddp import native
+
+    C = native()
+    with pytest.raises(RuntimeError):
+        C.linear_int8(0, 16, 0, 0, 16, 0, 0, 0, 0, 4, 4, 2**17, False, 0)
+    with pytest.raises(RuntimeError):
+        C.linear_int8(0, 16, 0, 0, 16, 0, 0, 0, 0, 4, 0, 16, False, 0)
+    with pytest.raises(RuntimeError):
+        C.quantize_rows(0, 0, 16, 0, 8, 0, 4, 16, 0)
+    with pytest.raises(RuntimeError):
+        C.quantize_rows(0, 3, 16, 0, 16, 0, 4, 16, 0)
+    x = torch.randn(2, 8, device=cuda)
+    with pytest.raises(ValueError):
+        ops.linear_int8(x, torch.zeros(3, 8, dtype=torch.int8), torch.ones(3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 24, 300])
+def test_linear_int8_stream_and_graph(cuda, M):
+    """On another stream, and captured: two graphs that replay in turn with new inputs."""
+    N, K = 200, 520
+    x, w, ws, b = make(M, N, K, torch.bfloat16)
+    xg, wg, wsg, bg = (t.to(cuda) for t in (x, w, ws, b))
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        y = ops.linear_int8(xg, wg, wsg, bg)
+    st.synchronize()
+    q, s = oracle_quantize(x)
+    check_linear(y, q, s, w, ws, b, False)
+    graphs = []
+    for _ in range(2):
+        xin = xg.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.linear_int8(xin, wg, wsg, bg)
+        graphs.append((g, xin, out))
+    for i in range(3):
+        for j, (g, xin, out) in enumerate(graphs):
+            xin.copy_(xg * (1 + i + 3 * j))
+            g.replay()
+        for j, (g, xin, out) in enumerate(graphs):
+            assert torch.equal(out, ops.linear_int8(xin, wg, wsg, bg)), (i, j)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("bias,relu,K", [(True, True, 100), (False, False, 64), (True, False, 33)])
+def test_int8_linear_layer(dev, bias, relu, K):
+    """Int8Linear.from_linear: the layer's weight in int8, its outputs those of ops.linear_int8."""
+    torch.manual_seed(0)
+    lin = Linear(K, 30, bias=bias, fuse_relu=relu).to(dev)
+    lay = Int8Linear.from_linear(lin)
+    wq, ws = oracle_quantize(lin.weight)
+    assert torch.equal(lay.weight[:, :K].cpu(), wq) and torch.equal(lay.weight_scale.cpu(), ws)
+    x = torch.randn(5, 2, K)
+    q, s = oracle_quantize(x.reshape(10, K))
+    with torch.no_grad():
+        y = lay(x.to(dev))
+    b = lin.bias.detach().cpu() if bias else None
+    check_linear(y.reshape(10, 30), q, s, wq, ws, b, relu)
+    other = Int8Linear(K, 30, bias=bias, fuse_relu=relu).to(dev)
+    other.load_state_dict(lay.state_dict())
+    with torch.no_grad():
+        assert torch.equal(other(x.to(dev)), y)
+    assert sum(p.numel() for p in lay.parameters()) == 0
