@@ -273,10 +273,11 @@ PYBIND11_MODULE(_C, m) {
                 P<const float>(bias), P<void>(y), ytype, M, N, K, relu, S(st));
   });
   m.def("top_logits", [](uintptr_t z, int type, int64_t ldz, int64_t rows, int V, int k, double temperature,
-                         uintptr_t values, uintptr_t index, uintptr_t lse, uintptr_t st) {
+                         uintptr_t values, uintptr_t index, uintptr_t lse, uintptr_t scratch, uintptr_t st) {
     top_logits(P<const void>(z), type, ldz, rows, V, k, temperature, P<void>(values), P<int32_t>(index),
-               P<float>(lse), S(st));
+               P<float>(lse), P<void>(scratch), S(st));
   });
+  m.def("top_logits_scratch", &top_logits_scratch);
   m.def("distill_fwd", [](uintptr_t z, uintptr_t tv, uintptr_t ti, uintptr_t target, uintptr_t tlse, uintptr_t stats,
                           int64_t ldz, int64_t rows, int V, int k, int type, int tv_type, bool ti64, bool target64,
                           double temperature, double hard, uintptr_t loss_rows, uintptr_t loss, bool mean,

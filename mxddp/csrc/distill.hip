@@ -13,6 +13,8 @@
 // The bracketed terms belong to a given teacher lse; S = sum_j p_j [+ r].  The classes outside keep a maximum and a sum of
 // their own, so what they hold is never the difference of two near numbers, and a row's exponentials
 // are taken relative to that maximum: none of them overflows.
+#include <algorithm>
+
 #include "lowp.h"
 #include "ops.h"
 
@@ -33,26 +35,33 @@ __device__ __forceinline__ uint64_t order_key(float v, uint32_t i) {
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
 
+// v_exp_f32 alone: results below 2^-126 are 0
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // running (maximum, sum of exp2((z - m) c))
 struct MaxSum {
   float m = kLowest, s = 0.f;
-  __device__ __forceinline__ void add(float z, float c) {
+  __device__ __forceinline__ void raise(float z, float c) {
     if (z > m) {
-      s *= exp2f((m - z) * c);
+      s *= exp2_raw((m - z) * c);
       m = z;
     }
-    s += exp2f((z - m) * c);
+  }
+  __device__ __forceinline__ void add(float z, float c) {
+    raise(z, c);
+    s += exp2_raw((z - m) * c);
   }
   __device__ __forceinline__ void merge(float om, float os, float c) {
     const float n = fmaxf(m, om);
-    s = s * exp2f((m - n) * c) + os * exp2f((om - n) * c);
+    s = s * exp2_raw((m - n) * c) + os * exp2_raw((om - n) * c);
     m = n;
   }
 };
 
 constexpr int kT = 256;
 
-// over a block of kT threads; every thread gets the result
+// over a block of TB threads; every thread gets the result
+template <int TB>
 __device__ __forceinline__ MaxSum block_merge(MaxSum v, float c, float* red) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -66,50 +75,307 @@ __device__ __forceinline__ MaxSum block_merge(MaxSum v, float c, float* red) {
   }
   __syncthreads();
   MaxSum t;
-  for (int w = 0; w < kT / 64; ++w) t.merge(red[2 * w], red[2 * w + 1], c);
+  for (int w = 0; w < TB / 64; ++w) t.merge(red[2 * w], red[2 * w + 1], c);
   return t;
 }
 
-template <class T>
-__global__ __launch_bounds__(kT) void top_logits_k(const typename T::store_t* __restrict__ z, int64_t ldz, int V,
-                                                   int k, float c, float inv_t, typename T::store_t* __restrict__ val,
-                                                   int32_t* __restrict__ idx, float* __restrict__ lse) {
-  __shared__ float red[2 * kT / 64];
-  __shared__ uint64_t rk[kT / 64];
-  const int64_t row = blockIdx.x;
-  z += row * ldz;
-  MaxSum ms;
-  for (int i = threadIdx.x; i < V; i += kT) ms.add(T::load(z[i]), c);
-  ms = block_merge(ms, c, red);
-  uint64_t last = ~0ull;
-  for (int j = 0; j < k; ++j) {
-    uint64_t best = 0;
-    for (int i = threadIdx.x; i < V; i += kT) {
-      const uint64_t key = order_key(T::load(z[i]), i);
-      if (key < last && key > best) best = key;
-    }
+// ---------------------------------------------------------------------------- top logits
+// One pass over the row: a block of TB threads takes tiles of TB x kU pieces into registers, and of
+// each piece the maximum and the exponentials' sum.  In the first tile the threshold is the largest
+// 16-bit prefix of a value that at least k pieces' maxima reach, so at least k elements do, and for
+// independent values hardly more.  Elements that reach it become candidates in LDS; in later tiles an
+// element has to be above the threshold: one equal to it comes after k others that are as large.
+// When the list grows, its threshold is raised in the same way; where ties overflow it (constant or
+// sorted rows) the k largest keys of list and tile are selected exactly, bit by bit.  In the end a
+// candidate's place is the number of larger keys.
+//
+// Few long rows are split over blocks: each leaves its segment's k largest keys, in order, and its
+// sum, and top_merge_k joins them.
+constexpr int kU = 4;       // pieces of 16 bytes a thread holds
+// candidates: twice the largest k and more; a block of one wave has short rows, and many to a CU
+constexpr int top_cap(int tb) { return tb == 64 ? 512 : 1024; }
+
+struct TopArgs {
+  const void* z;
+  void* val;
+  int32_t* idx;
+  float* lse;
+  uint64_t* part;  // [rows][nseg][k] keys, 0 behind a segment's last; then [rows][nseg] (m, s)
+  int64_t ldz, rows;
+  int V, k, nseg, seglen;
+  float c, inv_t;
+};
+
+__device__ __forceinline__ int wave_count(bool b) { return __popcll(__ballot(b)); }
+// a block's total of its waves' counts.  `slots` holds two rounds, so one barrier a round is enough.
+template <int TB>
+__device__ __forceinline__ int block_count(int wave_total, int* slots, int round) {
+  if constexpr (TB == 64) return wave_total;
+  int* s = slots + (round & 1) * (TB / 64);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = wave_total;
+  __syncthreads();
+  int n = 0;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor((unsigned long long)best, o, 64);
-      best = other > best ? other : best;
+  for (int w = 0; w < TB / 64; ++w) n += s[w];
+  return n;
+}
+
+// the number whose order bits these are (0xffffffff: a NaN)
+__device__ __forceinline__ float from_order_bits(uint32_t b) {
+  return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+
+// The k largest of the n keys in `from` and of a tile's elements, [base, end) of z, go to `to`, in any
+// order; returns the smallest of them.  There must be k.  The tile is read again for every bit (from
+// the caches): taking it in registers would put every tile's registers in memory for this rare call.
+template <class T, int TB>
+__device__ __noinline__ uint64_t select_exact(const uint64_t* from, int n, uint64_t* to,
+                                              const typename T::store_t* z, int base, int end, int k, int* slots,
+                                              int* cnt) {
+  const int tid = threadIdx.x;
+  constexpr int N = Piece<T>::kN;
+  const int pieces = (max(end - base, 0) + N - 1) / N;
+  uint64_t t = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t trial = t | 1ull << bit;
+    int c = 0;
+    for (int i = tid; i < (n + 63) / 64 * 64; i += TB) c += wave_count(i < n && from[i] >= trial);
+    for (int p = tid; p < (pieces + 63) / 64 * 64; p += TB) {
+      const int i = base + p * N;
+      Piece<T> x;
+      x.load(z, i, end, T::kNegInf);
+#pragma unroll
+      for (int e = 0; e < N; ++e) c += wave_count(i + e < end && order_key(x.get(e), i + e) >= trial);
+    }
+    if (block_count<TB>(c, slots, bit) >= k) t = trial;
+  }
+  if (tid == 0) *cnt = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += TB)
+    if (from[i] >= t) to[atomicAdd(cnt, 1)] = from[i];
+  for (int i = base + tid; i < end; i += TB) {
+    const uint64_t key = order_key(T::load(z[i]), i);
+    if (key >= t) to[atomicAdd(cnt, 1)] = key;
+  }
+  __syncthreads();
+  return t;
+}
+
+// Candidates in LDS: two lists, the current one, its length, and what a further element has to exceed
+template <int TB>
+struct Candidates {
+  uint64_t* list;
+  uint64_t* other;
+  int* slots;
+  int* cnt;
+  int n;
+  float t;
+
+  // keep those that reach the largest 16-bit prefix that k of them reach
+  __device__ __forceinline__ void raise(int k) {
+    const int tid = threadIdx.x;
+    uint32_t prefix = 0;
+#pragma unroll 1
+    for (int bit = 15; bit >= 0; --bit) {
+      const uint32_t trial = prefix | 1u << bit;
+      int c = 0;
+      for (int i = tid; i < (n + 63) / 64 * 64; i += TB) c += wave_count(i < n && (uint32_t)(list[i] >> 48) >= trial);
+      if (block_count<TB>(c, slots, bit) >= k) prefix = trial;
+    }
+    if (tid == 0) *cnt = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += TB)
+      if ((uint32_t)(list[i] >> 48) >= prefix) other[atomicAdd(cnt, 1)] = list[i];
+    __syncthreads();
+    n = *cnt;
+    swap();
+    t = from_order_bits(prefix << 16);
+  }
+  __device__ __forceinline__ void swap() {
+    uint64_t* l = list;
+    list = other;
+    other = l;
+  }
+};
+
+// the row's rank-th answer; the first one's writer has the sum: an infinite or NaN maximum is its value
+template <class T>
+__device__ __forceinline__ void put_top(const TopArgs& a, int64_t row, int rank, uint64_t key,
+                                        const typename T::store_t* z, const MaxSum& ms) {
+  const uint32_t at = key_index(key);
+  static_cast<typename T::store_t*>(a.val)[row * a.k + rank] = z[at];
+  a.idx[row * a.k + rank] = (int32_t)at;
+  if (rank == 0) {
+    const float v = T::load(z[at]);
+    a.lse[row] = v - v == 0.f ? ms.m * a.inv_t + logf(ms.s) : v;
+  }
+}
+
+template <class T, int TB>
+__global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
+  constexpr int N = Piece<T>::kN, TILE = TB * kU * N, kCap = top_cap(TB);
+  static_assert(kCap >= 2 * kTopMax, "a list that was cut to k leaves half of its room");
+  __shared__ uint64_t buf[2][kCap];
+  __shared__ int slots[2 * TB / 64], cnt;
+  __shared__ float red[2 * TB / 64];
+  const int tid = threadIdx.x, k = a.k;
+  const int64_t row = blockIdx.x / a.nseg;
+  const int seg = blockIdx.x % a.nseg, begin = seg * a.seglen, end = min(a.V, begin + a.seglen);
+  const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
+  Candidates<TB> cand{buf[0], buf[1], slots, &cnt, 0, 0.f};
+  MaxSum ms;
+  if (tid == 0) cnt = 0;
+#pragma unroll 1
+  for (int base = begin; base < end; base += TILE) {
+    Piece<T> x[kU];
+    float top[kU];
+    bool odd[kU];  // the piece's sum is NaN: it may hold one, or infinities
+#pragma unroll
+    for (int u = 0; u < kU; ++u) x[u].load(z, base + (u * TB + tid) * N, end, T::kNegInf);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float m = x[u].get(0);
+#pragma unroll
+      for (int e = 1; e < N; ++e) m = fmaxf(m, x[u].get(e));
+      top[u] = m;
+      ms.raise(m, a.c);
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += exp2_raw((x[u].get(e) - ms.m) * a.c);
+      odd[u] = s != s;
+      ms.s += s;
+    }
+    const bool first = base == begin;
+    uint32_t prefix = 0;
+    if (first) {
+#pragma unroll 1
+      for (int bit = 15; bit >= 0; --bit) {
+        const uint32_t trial = prefix | 1u << bit;
+        int c = 0;
+#pragma unroll
+        for (int u = 0; u < kU; ++u)  // a piece of NaN alone counts as one
+          c += wave_count(base + (u * TB + tid) * N < end && order_bits(top[u]) >> 16 >= trial);
+        if (block_count<TB>(c, slots, bit) >= k) prefix = trial;
+      }
+      cand.t = from_order_bits(prefix << 16);
     }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) rk[threadIdx.x >> 6] = best;
-    __syncthreads();
-    for (int w = 0; w < kT / 64; ++w) best = rk[w] > best ? rk[w] : best;
-    last = best;
-    if (threadIdx.x == 0) {
-      const uint32_t i = key_index(best);
-      val[row * k + j] = z[i];
-      idx[row * k + j] = (int32_t)i;
-      if (j == 0) {
-        const float v = T::load(z[i]);
-        // an infinite or NaN maximum is the sum's value; of a row of -inf as well
-        const bool fin = v - v == 0.f;
-        lse[row] = fin ? ms.m * inv_t + logf(ms.s) : v;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int i0 = base + (u * TB + tid) * N;
+      if (odd[u] || (first ? order_bits(top[u]) >= prefix << 16 : top[u] > cand.t)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float v = x[u].get(e);
+          if (i0 + e < end && (first ? order_bits(v) >= prefix << 16 : !(v <= cand.t))) {
+            const int pos = atomicAdd(&cnt, 1);
+            if (pos < kCap) cand.list[pos] = order_key(v, i0 + e);
+          }
+        }
       }
     }
+    __syncthreads();
+    const int had = cand.n;
+    cand.n = cnt;
+    if (cand.n > kCap) {  // the exact k of the list before this tile and of the tile
+      const uint64_t low =
+          select_exact<T, TB>(cand.list, had, cand.other, z, base, min(end, base + TILE), k, slots, &cnt);
+      cand.t = from_order_bits((uint32_t)(low >> 32));
+      cand.swap();
+      cand.n = k;
+    } else if (cand.n > kCap / 2) {
+      __syncthreads();  // every thread has read cnt
+      cand.raise(k);
+      if (cand.n > kCap / 2) {
+        const uint64_t low = select_exact<T, TB>(cand.list, cand.n, cand.other, z, 0, 0, k, slots, &cnt);
+        cand.t = from_order_bits((uint32_t)(low >> 32));
+        cand.swap();
+        cand.n = k;
+      }
+    }
+    __syncthreads();
   }
+  ms = block_merge<TB>(ms, a.c, red);
+  if (cand.n > k + 64) cand.raise(k);
+  const int n = cand.n, kk = min(k, n);
+  for (int i = tid; i < n; i += TB) {
+    const uint64_t key = cand.list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += cand.list[j] > key;
+    if (rank >= kk) continue;
+    if (a.nseg == 1) put_top<T>(a, row, rank, key, z, ms);
+    else a.part[(row * a.nseg + seg) * k + rank] = key;
+  }
+  if (a.nseg > 1) {
+    for (int i = kk + tid; i < k; i += TB) a.part[(row * a.nseg + seg) * k + i] = 0;
+    if (tid == 0) reinterpret_cast<float2*>(a.part + a.rows * a.nseg * k)[row * a.nseg + seg] = make_float2(ms.m, ms.s);
+  }
+}
+
+// The k largest of a row's nseg sorted lists of k keys.  As many keys as k reach the smallest of the
+// lists' (k / nseg)-th, and the largest of their last: what is below either is out.
+template <class T>
+__global__ __launch_bounds__(kT) void top_merge_k(TopArgs a) {
+  constexpr int kCap = top_cap(kT);
+  __shared__ uint64_t buf[2][kCap];
+  __shared__ int slots[2 * kT / 64], cnt;
+  __shared__ float red[2 * kT / 64];
+  const int tid = threadIdx.x, k = a.k, total = a.nseg * k;
+  const int64_t row = blockIdx.x;
+  const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
+  const uint64_t* keys = a.part + row * total;
+  Candidates<kT> cand{buf[0], buf[1], slots, &cnt, 0, 0.f};
+  MaxSum ms;
+  const int each = (k + a.nseg - 1) / a.nseg;
+  uint64_t least = ~0ull, last = 0;
+  for (int s = 0; s < a.nseg; ++s) {
+    const uint64_t x = keys[s * k + each - 1], y = keys[s * k + k - 1];
+    least = x < least ? x : least;
+    last = y > last ? y : last;
+  }
+  const uint64_t floor = least > last ? least : last;
+  if (tid < a.nseg) {
+    const float2 p = reinterpret_cast<const float2*>(a.part + a.rows * total)[row * a.nseg + tid];
+    ms.m = p.x;
+    ms.s = p.y;
+  }
+  if (tid == 0) cnt = 0;
+  ms = block_merge<kT>(ms, a.c, red);
+  for (int i = tid; i < total; i += kT)
+    if (keys[i] >= floor && keys[i] != 0) {
+      const int pos = atomicAdd(&cnt, 1);
+      if (pos < kCap) cand.list[pos] = keys[i];
+    }
+  __syncthreads();
+  cand.n = cnt;
+  __syncthreads();
+  if (cand.n > kCap) {
+    select_exact<T, kT>(keys, total, cand.list, z, 0, 0, k, slots, &cnt);
+    cand.n = k;
+  } else if (cand.n > k + 64) {
+    cand.raise(k);
+  }
+  for (int i = tid; i < cand.n; i += kT) {
+    const uint64_t key = cand.list[i];
+    int rank = 0;
+    for (int j = 0; j < cand.n; ++j) rank += cand.list[j] > key;
+    if (rank < k) put_top<T>(a, row, rank, key, z, ms);
+  }
+}
+
+// blocks of a row: long rows that alone would not fill the machine are cut into pieces of 8,192
+// classes or more, one tile of a block of 256 threads for a 16-bit type
+int top_segments(int64_t rows, int V) {
+  const int64_t want = (2 * device_cu_count() + rows - 1) / std::max<int64_t>(rows, 1);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, (V + 8191) / 8192, 32}));
+}
+
+template <class T, int TB>
+void launch_top(const TopArgs& a, hipStream_t st) {
+  const int64_t blocks = a.rows * a.nseg;
+  MX_LAUNCH((top_logits_k<T, TB>), dim3((uint32_t)blocks), dim3(TB), 0, st, a);
 }
 
 __device__ __forceinline__ int64_t load_int(const void* p, int64_t i, int is64) {
@@ -187,13 +453,13 @@ __global__ __launch_bounds__(kT) void distill_fwd_k(DistillArgs a, float* __rest
       if (two) one.add(v, c1);
     }
   }
-  out = block_merge(out, c, red);
-  if (two) one = block_merge(one, c1, red);
+  out = block_merge<kT>(out, c, red);
+  if (two) one = block_merge<kT>(one, c1, red);
   // all classes: those outside and the named ones, each once
   MaxSum in;
   const float zc = cls >= 0 ? T::load(z[cls]) : 0.f;
   if (tail && first) in.add(zc, c);
-  in = block_merge(in, c, red);
+  in = block_merge<kT>(in, c, red);
   MaxSum all = out;
   if (tail) all.merge(in.m, in.s, c);
   if (two) { one.s *= exp2f((one.m - all.m) * c1); one.m = all.m; }
@@ -326,15 +592,32 @@ void check_distill(const DistillArgs& a) {
 
 }  // namespace
 
+int64_t top_logits_scratch(int64_t rows, int V, int k) {
+  const int nseg = top_segments(rows, V);
+  return nseg > 1 ? rows * nseg * (k + 1) : 0;
+}
+
 void top_logits(const void* z, int type, int64_t ldz, int64_t rows, int V, int k, double temperature, void* values,
-                int32_t* index, float* lse, hipStream_t st) {
+                int32_t* index, float* lse, void* scratch, hipStream_t st) {
   MX_CHECK(rows >= 0 && rows < (1ll << 31) && V >= 1 && V <= (1 << 30) && k >= 1 && k <= kTopMax && k <= V &&
                temperature > 0,
            "top_logits: bad sizes");
   if (rows == 0) return;
-  MX_BY_TYPE(type, T, MX_LAUNCH(top_logits_k<T>, dim3((uint32_t)rows), dim3(kT), 0, st,
-                                static_cast<const typename T::store_t*>(z), ldz, V, k, (float)(kLog2e / temperature),
-                                (float)(1.0 / temperature), static_cast<typename T::store_t*>(values), index, lse));
+  TopArgs a{z, values, index, lse, static_cast<uint64_t*>(scratch), ldz, rows, V, k, top_segments(rows, V), V,
+            (float)(kLog2e / temperature), (float)(1.0 / temperature)};
+  if (a.nseg > 1) {
+    MX_CHECK(scratch, "top_logits: long rows need scratch");
+    a.seglen = (cdiv(V, a.nseg) + 63) / 64 * 64;
+    a.nseg = cdiv(V, a.seglen);
+  }
+  // one tile where a block's part of the row fits: a wave alone needs no barrier
+  MX_BY_TYPE(type, T, {
+    constexpr int wave_tile = 64 * kU * Piece<T>::kN;
+    if (a.seglen <= wave_tile) launch_top<T, 64>(a, st);
+    else if (a.seglen <= 4 * wave_tile) launch_top<T, 256>(a, st);
+    else launch_top<T, 512>(a, st);
+    if (a.nseg > 1) MX_LAUNCH(top_merge_k<T>, dim3((uint32_t)rows), dim3(kT), 0, st, a);
+  });
 }
 
 void distill_fwd(const DistillArgs& a, float* loss_rows, float* loss, bool mean, hipStream_t st) {

@@ -306,8 +306,10 @@ void linear_int8(const int8_t* q, int64_t ldq, const float* xs, const int8_t* w,
 constexpr int kTopMax = 256;  // most top logits of a row
 // the k largest logits of each row in falling order (equal ones by index), their indices, and
 // lse = log sum exp(z / temperature)
+// scratch: top_logits_scratch(...) words of 8 bytes (0: none needed)
+int64_t top_logits_scratch(int64_t rows, int V, int k);
 void top_logits(const void* z, int type, int64_t ldz, int64_t rows, int V, int k, double temperature, void* values,
-                int32_t* index, float* lse, hipStream_t st);
+                int32_t* index, float* lse, void* scratch, hipStream_t st);
 struct DistillArgs {
   const void* z;        // [rows][ldz] student logits
   const void* tv;       // [rows][k] teacher logits

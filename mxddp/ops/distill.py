@@ -61,8 +61,11 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     index = torch.empty((*lead, k), device=z.device, dtype=torch.int32)
     lse = torch.empty(lead, device=z.device, dtype=torch.float32)
     with on_device(z):
-        native().top_logits(z.data_ptr(), DTYPES[z.dtype], z.stride(0), rows, V, k, temperature, values.data_ptr(),
-                            index.data_ptr(), lse.data_ptr(), stream_of(z))
+        C = native()
+        n = C.top_logits_scratch(rows, V, k)
+        scratch = torch.empty((n,), device=z.device, dtype=torch.int64) if n else None
+        C.top_logits(z.data_ptr(), DTYPES[z.dtype], z.stride(0), rows, V, k, temperature, values.data_ptr(),
+                     index.data_ptr(), lse.data_ptr(), _p(scratch), stream_of(z))
     return TopLogits(values, index, lse)
 
 

@@ -451,11 +451,11 @@ def test_refusals_native(cuda):
 
     C = native()
     with pytest.raises(RuntimeError):
-        C.top_logits(0, 0, 8, 2, 8, 9, 1.0, 0, 0, 0, 0)
+        C.top_logits(0, 0, 8, 2, 8, 9, 1.0, 0, 0, 0, 0, 0)
     with pytest.raises(RuntimeError):
-        C.top_logits(0, 0, 400, 2, 400, 257, 1.0, 0, 0, 0, 0)
+        C.top_logits(0, 0, 400, 2, 400, 257, 1.0, 0, 0, 0, 0, 0)
     with pytest.raises(RuntimeError):
-        C.top_logits(0, 5, 8, 2, 8, 2, 1.0, 0, 0, 0, 0)
+        C.top_logits(0, 5, 8, 2, 8, 2, 1.0, 0, 0, 0, 0, 0)
     with pytest.raises(RuntimeError):
         C.distill_fwd(0, 0, 0, 0, 0, 0, 8, 2, 8, 300, 0, 0, False, False, 1.0, 0.0, 0, 0, True, 0)
     with pytest.raises(RuntimeError):
