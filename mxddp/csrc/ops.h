@@ -294,6 +294,7 @@ void augment_crop_flip_norm(const float* x, float* y, int N, int C, int H, int W
 // ---- linear layers in 8-bit integers (int8_linear.hip); element types: lowp.h DType ----
 // |q w| <= 2^14, so up to this many products sum to less than 2^31
 constexpr int kInt8MaxK = (1 << 17) - 1;
+constexpr int64_t kInt8MaxLd = 1 << 22;  // largest row stride: a tile's rows are within 32 bits
 // q [rows][ldq] int8 (columns K .. ldq - 1 zeroed), scale [rows]: x ~ q * scale, scale = max|x| / 127
 // (at least 2^-126; NaN, with q = 0, for a row that is not finite)
 void quantize_rows(const void* x, int xtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K,

@@ -15,6 +15,7 @@ from .lowp import DTYPES, MAX_ROWS, check_device, check_float, on_device, rows_o
 
 MAX_K = 2**17 - 1  # products of 2^14 each whose sum stays below 2^31
 _TINY = 2.0**-126
+_MAX_LD = 2**22      # csrc/ops.h kInt8MaxLd
 
 
 def quantize_rows(x: torch.Tensor):
@@ -94,9 +95,11 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     M = x2.shape[0]
     if M > MAX_ROWS:
         raise ValueError(f"linear_int8: {M} rows, at most {MAX_ROWS}")
-    weight = weight if weight.stride(1) == 1 or K == 1 else weight.contiguous()
+    if (weight.stride(1) != 1 and K > 1) or weight.stride(0) > _MAX_LD:
+        weight = weight.contiguous()
     y = torch.empty((*x.shape[:-1], N), device=x.device, dtype=out_dtype)
     if given:
+        x2 = x2 if x2.stride(0) <= _MAX_LD else x2.contiguous()
         q, ldq, s = x2, x2.stride(0), x_scale.contiguous()
     else:
         ldq = (K + 15) // 16 * 16

@@ -173,6 +173,9 @@ def test_linear_int8_strides(dev, M):
         qv.copy_(q)
         y = ops.linear_int8(qv, wv, ws.to(dev), b.to(dev), x_scale=s.to(dev))
         check_linear(y, q, s, w, ws, b, False)
+    far = torch.zeros(N, 2**22 + 16, dtype=torch.int8, device=dev)[:, :K]  # rows further apart than a tile's offsets
+    far.copy_(w)
+    check_linear(ops.linear_int8(x.to(dev), far, ws.to(dev)), q, s, w, ws, None, False)
     # the weight's rows stored column by column; an input of more dimensions; every second scale
     wt = w.to(dev).t().contiguous().t()
     ws2 = torch.stack([ws, ws + 1], 1).to(dev)[:, 0]
