@@ -267,10 +267,11 @@ PYBIND11_MODULE(_C, m) {
                             int64_t rows, int K, uintptr_t st) {
     quantize_rows(P<const void>(x), xtype, ldx, P<int8_t>(q), ldq, P<float>(scale), rows, K, S(st));
   });
-  m.def("linear_int8", [](uintptr_t q, int64_t ldq, uintptr_t xs, uintptr_t w, int64_t ldw, uintptr_t ws,
-                          uintptr_t bias, uintptr_t y, int ytype, int64_t M, int N, int K, bool relu, uintptr_t st) {
-    linear_int8(P<const int8_t>(q), ldq, P<const float>(xs), P<const int8_t>(w), ldw, P<const float>(ws),
-                P<const float>(bias), P<void>(y), ytype, M, N, K, relu, S(st));
+  m.def("linear_int8", [](uintptr_t q, int64_t ldq, int q_room, uintptr_t xs, uintptr_t w, int64_t ldw, int w_room,
+                          uintptr_t ws, uintptr_t bias, uintptr_t y, int ytype, int64_t M, int N, int K, bool relu,
+                          uintptr_t st) {
+    linear_int8(P<const int8_t>(q), ldq, q_room, P<const float>(xs), P<const int8_t>(w), ldw, w_room,
+                P<const float>(ws), P<const float>(bias), P<void>(y), ytype, M, N, K, relu, S(st));
   });
   m.def("top_logits", [](uintptr_t z, int type, int64_t ldz, int64_t rows, int V, int k, double temperature,
                          uintptr_t values, uintptr_t index, uintptr_t lse, uintptr_t scratch, uintptr_t st) {

@@ -105,6 +105,24 @@ __device__ __forceinline__ i32x4 row16(const int8_t* p, bool row_ok, int k, int 
   return v;
 }
 
+// 16 bytes at any address
+__device__ __forceinline__ i32x4 load16(const int8_t* p) {
+  const Bytes16 b = *reinterpret_cast<const Bytes16*>(p);
+  return i32x4{(int)b.v[0], (int)b.v[1], (int)b.v[2], (int)b.v[3]};
+}
+
+// A piece that reaches `over` bytes behind the end of a row was read that much before its place, at
+// the row's last 16 bytes: move it there, with zeros behind the end.
+__device__ __forceinline__ i32x4 tail16(i32x4 v, int over) {
+  if (over >= 16) return i32x4{0, 0, 0, 0};
+  if (over <= 0) return v;
+  if (over & 8) v = i32x4{v[2], v[3], 0, 0};
+  if (over & 4) v = i32x4{v[1], v[2], v[3], 0};
+  const uint32_t b = over & 3;
+  return i32x4{(int)__builtin_amdgcn_alignbyte(v[1], v[0], b), (int)__builtin_amdgcn_alignbyte(v[2], v[1], b),
+               (int)__builtin_amdgcn_alignbyte(v[3], v[2], b), (int)__builtin_amdgcn_alignbyte(0, v[3], b)};
+}
+
 struct GemmArgs {
   const int8_t* q;
   const int8_t* w;
@@ -116,23 +134,67 @@ struct GemmArgs {
   int N, K, relu, tiles_n, tiles_m;
 };
 
-__device__ uint4 g_zero16;
+// the epilogue of four channels of a token: their scales and biases, once for all tokens of a lane
+struct Four {
+  float ws[4], b[4];
+  __device__ __forceinline__ Four(const GemmArgs& a, int n) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = min(n + e, a.N - 1);
+      ws[e] = a.ws[c];
+      b[e] = a.bias ? a.bias[c] : 0.f;
+    }
+  }
+  template <class T>
+  __device__ __forceinline__ void put(const GemmArgs& a, int64_t m, int n, i32x4 acc, float xs) const {
+    typename T::store_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float f = (float)acc[e] * xs * ws[e] + b[e];
+      v[e] = T::store(a.relu && f < 0.f ? 0.f : f);  // a NaN stays one
+    }
+    typename T::store_t* o = static_cast<typename T::store_t*>(a.y) + m * a.N + n;
+    if (n + 3 < a.N) {
+      __builtin_memcpy(o, v, sizeof(v));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.N) o[e] = v[e];
+    }
+  }
+};
+
 typedef __attribute__((address_space(3))) void lds_void_t;
-__device__ __forceinline__ void glds16(const void* src, void* lds) {
-  __builtin_amdgcn_global_load_lds(src, (lds_void_t*)lds, 16, 0, 0);
+// 16 bytes a lane straight to LDS (lane after lane from `lds`), from base + off.  A buffer instruction:
+// the compiler takes a global one for an access through the flat path, which may touch LDS in any
+// order, and would then wait for ALL of a wave's LDS reads before each use of one.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00027000);
+}
+__device__ __forceinline__ void glds16(__amdgpu_buffer_rsrc_t r, uint32_t off, int k0, void* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)lds, 16, (int)off, k0, 0, 0);
 }
 
-// TM channels x TN tokens per block of WM x WN waves, 128 k a stage, two stages in LDS.  A stage's
-// rows are 128 bytes, a row's 16-byte pieces XOR-permuted by its number, so the fragments' reads (16
-// rows at one piece) spread over all banks.  DMA: the stage comes straight from global memory
-// (rows of whole, aligned pieces); else through registers (any alignment, the ragged end of k in
-// bytes).  Channels are the matrix instruction's rows: a lane ends with four of them for one token.
-template <class T, int TM, int TN, int WM, int WN, bool DMA>
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// TM channels x TN tokens per block of WM x WN waves, 128 k a stage, NS stages in LDS.  A stage's rows
+// are 128 bytes, a row's 16-byte pieces XOR-permuted by its number, so the fragments' reads (16 rows at
+// one piece) spread over all banks.  DW, DQ: the channels' and the tokens' rows come straight from
+// global memory (rows of whole, aligned pieces); else through registers (any alignment and K >= 16).  Channels are the matrix instruction's rows: a lane ends with four of them for one
+// token.
+// The fragments of one half stage are read while the other half's are multiplied.  The barrier stands
+// in the middle of a stage, where its second half is in registers: its buffer is free for stage
+// t + NS there, and the first half of stage t + 1 is read behind it.
+template <class T, int TM, int TN, int WM, int WN, int NS, bool DW, bool DQ>
 __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
   constexpr int NW = WM * WN, FM = TM / WM / 16, FN = TN / WN / 16;
   constexpr int IA = TM / 8 / NW, IB = TN / 8 / NW;  // wave-wide copies of 1 KB a stage
   constexpr int SB = (TM + TN) * 128;
-  __shared__ __attribute__((aligned(1024))) char sm[2 * SB];
+  static_assert((DW && DQ) || NS == 2, "through registers one stage is under way");
+  __shared__ __attribute__((aligned(1024))) char sm[NS * SB];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
   const int bid = xcd_remap(blockIdx.x, gridDim.x);
   // tiles in bands of kBand channel tiles, token by token: what runs together shares both operands
@@ -152,111 +214,209 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
   for (int j = 0; j < IB; ++j)
     offq[j] = (uint32_t)(min<int64_t>((wave * IB + j) * 8 + (lane >> 3), a.M - 1 - m0) * a.ldq) + chunk;
 
-  i32x4 rw[DMA ? 1 : IA], rq[DMA ? 1 : IB];
-  auto fetch = [&](int t) {
+  const auto rsw = tile_rsrc(wbase), rsq = tile_rsrc(qbase);
+  i32x4 rw[DW ? 1 : IA], rq[DQ ? 1 : IB];
+  // straight to LDS
+  auto fetch = [&](int t, int buf) {
     const int k0 = t * 128;
-    if constexpr (DMA) {
-      char* st = sm + (t & 1) * SB;
-      if (k0 + 128 <= a.K) {
+    // pieces behind the end of k are the stage's first: `read` clears the tokens' side of them
+    const uint32_t back = k0 + chunk < a.K ? 0 : chunk;
+    char* st = sm + buf * SB;
 #pragma unroll
-        for (int j = 0; j < IA; ++j) glds16(wbase + k0 + offw[j], st + (wave * IA + j) * 1024);
+    for (int j = 0; j < (DW ? IA : 0); ++j) glds16(rsw, offw[j] - back, k0, st + (wave * IA + j) * 1024);
 #pragma unroll
-        for (int j = 0; j < IB; ++j) glds16(qbase + k0 + offq[j], st + TM * 128 + (wave * IB + j) * 1024);
-      } else {
-        const bool ok = k0 + chunk < a.K;
-        const void* zero = &g_zero16;
+    for (int j = 0; j < (DQ ? IB : 0); ++j)
+      glds16(rsq, offq[j] - back, k0, st + TM * 128 + (wave * IB + j) * 1024);
+  };
+  // to registers, and from there to LDS
+  auto load = [&](int t) {
+    const int at = min(t * 128 + chunk, a.K - 16) - chunk;
 #pragma unroll
-        for (int j = 0; j < IA; ++j) glds16(ok ? wbase + k0 + offw[j] : zero, st + (wave * IA + j) * 1024);
+    for (int j = 0; j < (DW ? 0 : IA); ++j) rw[j] = load16(wbase + at + offw[j]);
 #pragma unroll
-        for (int j = 0; j < IB; ++j) glds16(ok ? qbase + k0 + offq[j] : zero, st + TM * 128 + (wave * IB + j) * 1024);
-      }
-    } else {
+    for (int j = 0; j < (DQ ? 0 : IB); ++j) rq[j] = load16(qbase + at + offq[j]);
+  };
+  auto put = [&](int t, int buf) {
+    char* st = sm + buf * SB + lane * 16;
+    const int over = t * 128 + 128 > a.K ? t * 128 + chunk + 16 - a.K : 0;
+    auto to = [&](char* p, i32x4 v) {
+      if (t * 128 + 128 > a.K) v = tail16(v, over);
+      *reinterpret_cast<i32x4*>(p) = v;
+    };
 #pragma unroll
-      for (int j = 0; j < IA; ++j) rw[j] = row16(wbase + (offw[j] - chunk), true, k0 + chunk, a.K);
+    for (int j = 0; j < (DW ? 0 : IA); ++j) to(st + (wave * IA + j) * 1024, rw[j]);
 #pragma unroll
-      for (int j = 0; j < IB; ++j) rq[j] = row16(qbase + (offq[j] - chunk), true, k0 + chunk, a.K);
+    for (int j = 0; j < (DQ ? 0 : IB); ++j) to(st + TM * 128 + (wave * IB + j) * 1024, rq[j]);
+  };
+  const int fr = lane & 15, fc = lane >> 4;
+  const int rw0 = (wm * FM * 16 + fr) * 128, rq0 = TM * 128 + (wn * FN * 16 + fr) * 128;
+  auto read = [&](int t, int buf, int half, i32x4* fw, i32x4* fq) {
+    const char* st = sm + buf * SB + 16 * ((4 * half + fc) ^ (fr & 7));
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fw[i] = *reinterpret_cast<const i32x4*>(st + rw0 + i * 2048);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fq[j] = *reinterpret_cast<const i32x4*>(st + rq0 + j * 2048);
+    if (DQ && t * 128 + 128 > a.K) {
+      const bool ok = t * 128 + 64 * half + 16 * fc < a.K;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fq[j] = ok ? fq[j] : i32x4{0, 0, 0, 0};
     }
   };
-  auto put = [&](int t) {
-    if constexpr (!DMA) {
-      char* st = sm + (t & 1) * SB + lane * 16;
+  i32x4 acc[FM][FN] = {};
+  auto mul = [&](const i32x4* fw, const i32x4* fq) {
 #pragma unroll
-      for (int j = 0; j < IA; ++j) *reinterpret_cast<i32x4*>(st + (wave * IA + j) * 1024) = rw[j];
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < IB; ++j) *reinterpret_cast<i32x4*>(st + TM * 128 + (wave * IB + j) * 1024) = rq[j];
-    }
+      for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fq[j], acc[i][j], 0, 0, 0);
   };
 
-  i32x4 acc[FM][FN] = {};
   const int nt = (a.K + 127) / 128;
-  fetch(0);
-  put(0);
-  const int fr = lane & 15, fc = lane >> 4;
-  for (int t = 0; t < nt; ++t) {
-    if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // stage t is there for every wave, and stage t - 1 is used up
-    if (t + 1 < nt) fetch(t + 1);
-    const char* sw = sm + (t & 1) * SB + (wm * FM * 16 + fr) * 128;
-    const char* sq = sm + (t & 1) * SB + TM * 128 + (wn * FN * 16 + fr) * 128;
+  // through registers a stage is loaded behind the barrier before its turn and put in its place in the
+  // middle of the stage before it; the last stage is loaded again rather than under a condition, which
+  // would make the compiler wait for it at once
+  constexpr bool kDma = DW && DQ;
+  constexpr int kAhead = kDma ? NS : 2;
+  if constexpr (kDma) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const int c = 16 * ((4 * ks + fc) ^ (fr & 7));
-      i32x4 fw[FM], fq[FN];
-#pragma unroll
-      for (int i = 0; i < FM; ++i) fw[i] = *reinterpret_cast<const i32x4*>(sw + i * 2048 + c);
-#pragma unroll
-      for (int j = 0; j < FN; ++j) fq[j] = *reinterpret_cast<const i32x4*>(sq + j * 2048 + c);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fq[j], acc[i][j], 0, 0, 0);
-    }
-    if (t + 1 < nt) put(t + 1);
+    for (int s = 0; s < NS; ++s)
+      if (s < nt) fetch(s, s);
+    if (nt >= NS) wait_vm<(NS - 1) * (IA + IB)>();
+    else wait_vm<0>();
+  } else {
+    fetch(0, 0);
+    load(0);
+    put(0, 0);
+    wait_vm<0>();
+    if (nt > 1) fetch(1, 1);
+    load(min(1, nt - 1));
   }
-  typename T::store_t* y = static_cast<typename T::store_t*>(a.y);
+  lds_barrier();
+  i32x4 w0[FM], q0[FN], w1[FM], q1[FN];
+  read(0, 0, 0, w0, q0);
+  int buf = 0;
+  for (int t = 0; t < nt; ++t) {
+    const int next = buf + 1 == NS ? 0 : buf + 1;
+    read(t, buf, 1, w1, q1);
+    mul(w0, q0);
+    if (t + 1 < nt) {
+      if constexpr (kDma) {  // stage t + 1 has landed; up to NS - 2 later ones are under way
+        if (t + NS <= nt) wait_vm<(NS - 2) * (IA + IB)>();
+        else wait_vm<0>();
+      } else {
+        put(t + 1, next);
+        wait_vm<0>();
+      }
+      lds_barrier();
+      if (t + kAhead < nt) fetch(t + kAhead, buf);
+      if constexpr (!kDma) load(min(t + 2, nt - 1));
+      read(t + 1, next, 0, w0, q0);
+    }
+    mul(w1, q1);
+    buf = next;
+  }
+  float xs[FN];
+#pragma unroll
+  for (int j = 0; j < FN; ++j) xs[j] = a.xs[min<int64_t>(m0 + (wn * FN + j) * 16 + fr, a.M - 1)];
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int n = n0 + (wm * FM + i) * 16 + 4 * fc;
-    float ws[4], b[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      ws[e] = n + e < a.N ? a.ws[n + e] : 0.f;
-      b[e] = a.bias && n + e < a.N ? a.bias[n + e] : 0.f;
-    }
+    if (n >= a.N) continue;
+    const Four four(a, n);
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int64_t m = m0 + (wn * FN + j) * 16 + fr;
-      if (m >= a.M) continue;
-      const float xs = a.xs[m];
-      typename T::store_t v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float f = (float)acc[i][j][e] * xs * ws[e] + b[e];
-        v[e] = T::store(a.relu && f < 0.f ? 0.f : f);  // a NaN stays one
-      }
-      typename T::store_t* o = y + m * a.N + n;
-      if (n + 3 < a.N) {
-        __builtin_memcpy(o, v, sizeof(v));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < a.N) o[e] = v[e];
-      }
+      if (m < a.M) four.put<T>(a, m, n, acc[i][j], xs[j]);
     }
   }
 }
 
-template <class T, int TM, int TN, int WM, int WN>
-void launch_gemm(GemmArgs a, bool dma, hipStream_t st) {
+template <class T, int TM, int TN, int WM, int WN, int NS>
+void launch_gemm(GemmArgs a, bool dw, bool dq, hipStream_t st) {
   a.tiles_n = cdiv(a.N, TM);
   const int64_t tm = (a.M + TN - 1) / TN;
   MX_CHECK(tm * a.tiles_n < (1ll << 31) / 8, "linear_int8: too many tiles");
   a.tiles_m = (int)tm;
   const dim3 grid((uint32_t)(tm * a.tiles_n)), block(64 * WM * WN);
-  if (dma) MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, true>), grid, block, 0, st, a);
-  else MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, false>), grid, block, 0, st, a);
+  if (dw && dq) MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, NS, true, true>), grid, block, 0, st, a);
+  else if constexpr (TM * TN <= 128 * 128) {  // a larger tile's registers do not hold a stage as well
+    if (dq) MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, 2, false, true>), grid, block, 0, st, a);
+    else MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, 2, false, false>), grid, block, 0, st, a);
+  }
+}
+
+// Few tokens: bound by the weight's bytes.  A block of eight waves takes 16 FM channels and all of up
+// to 16 FN tokens; each wave streams an eighth of k from global memory straight into the matrix
+// instruction's operands (a lane has 16 bytes of one channel, 64 bytes of it lie in one instruction)
+// and the sums, whole numbers, are added in LDS.  The tokens' rows are small and come from the caches.
+constexpr int kSkinnyWaves = 8;
+
+template <class T, int FM, int FN>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void int8_skinny_k(GemmArgs a) {
+  __shared__ i32x4 part[kSkinnyWaves][FM * FN][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fc = lane >> 4;
+  const int n0 = (blockIdx.x % a.tiles_n) * 16 * FM;
+  const int64_t m0 = (int64_t)(blockIdx.x / a.tiles_n) * 16 * FN;
+  const int8_t *pw[FM], *pq[FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) pw[i] = a.w + (int64_t)min(n0 + 16 * i + fr, a.N - 1) * a.ldw + 16 * fc;
+#pragma unroll
+  for (int j = 0; j < FN; ++j) pq[j] = a.q + min<int64_t>(m0 + 16 * j + fr, a.M - 1) * a.ldq + 16 * fc;
+  i32x4 acc[FM][FN] = {};
+  const int units = (a.K + 63) / 64, whole = a.K / 64;
+  const int u0 = (int)((int64_t)units * wave / kSkinnyWaves), u1 = (int)((int64_t)units * (wave + 1) / kSkinnyWaves);
+  constexpr int U = 8 / FN < 2 ? 2 : 8 / FN;  // units in flight
+  int u = u0;
+  for (; u + U <= min(u1, whole); u += U) {
+    i32x4 fw[U][FM], fq[U][FN];
+#pragma unroll
+    for (int s = 0; s < U; ++s) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fw[s][i] = load16(pw[i] + 64 * (u + s));
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fq[s][j] = load16(pq[j] + 64 * (u + s));
+    }
+#pragma unroll
+    for (int s = 0; s < U; ++s)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[s][i], fq[s][j], acc[i][j], 0, 0, 0);
+  }
+  for (; u < u1; ++u) {  // what is left, the ragged end of k among it
+    i32x4 fw[FM], fq[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fw[i] = row16(pw[i] - 16 * fc, true, 64 * u + 16 * fc, a.K);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fq[j] = row16(pq[j] - 16 * fc, true, 64 * u + 16 * fc, a.K);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fq[j], acc[i][j], 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) part[wave][i * FN + j][lane] = acc[i][j];
+  __syncthreads();
+  for (int f = tid; f < FM * FN * 64; f += 64 * kSkinnyWaves) {
+    const int g = f >> 6, l = f & 63, i = g / FN, j = g % FN;
+    i32x4 v = part[0][g][l];
+#pragma unroll
+    for (int w = 1; w < kSkinnyWaves; ++w) v += part[w][g][l];
+    const int64_t m = m0 + 16 * j + (l & 15);
+    const int n = n0 + 16 * i + 4 * (l >> 4);
+    if (m < a.M && n < a.N) Four(a, n).put<T>(a, m, n, v, a.xs[m]);
+  }
+}
+
+template <class T, int FM, int FN>
+void launch_skinny(GemmArgs a, hipStream_t st) {
+  a.tiles_n = cdiv(a.N, 16 * FM);
+  const int64_t blocks = (a.M + 16 * FN - 1) / (16 * FN) * a.tiles_n;
+  MX_CHECK(blocks < (1ll << 31), "linear_int8: too many tiles");
+  MX_LAUNCH((int8_skinny_k<T, FM, FN>), dim3((uint32_t)blocks), dim3(64 * kSkinnyWaves), 0, st, a);
 }
 
 }  // namespace
@@ -276,17 +436,36 @@ void quantize_rows(const void* x, int xtype, int64_t ldx, int8_t* q, int64_t ldq
   });
 }
 
-void linear_int8(const int8_t* q, int64_t ldq, const float* xs, const int8_t* w, int64_t ldw, const float* ws,
-                 const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu, hipStream_t st) {
+void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, const int8_t* w, int64_t ldw, int w_room,
+                 const float* ws, const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu,
+                 hipStream_t st) {
   MX_CHECK(M >= 0 && N >= 1 && K >= 1 && K <= kInt8MaxK, "linear_int8: bad sizes");
   MX_CHECK(ldq >= 0 && ldq <= kInt8MaxLd && ldw >= 0 && ldw <= kInt8MaxLd, "linear_int8: row stride too large");
   if (M == 0) return;
   GemmArgs a{q, w, xs, ws, bias, y, ldq, ldw, M, N, K, relu ? 1 : 0, 0, 0};
-  auto whole = [](const void* p, int64_t ld) { return ((uintptr_t)p | (uintptr_t)ld) % 16 == 0; };
-  const bool dma = K % 16 == 0 && whole(q, ldq) && whole(w, ldw);
+  auto whole = [K](const void* p, int64_t ld, int room) {
+    return ((uintptr_t)p | (uintptr_t)ld) % 16 == 0 && room >= (K + 15) / 16 * 16;
+  };
+  const bool dw = whole(w, ldw, w_room), dq = whole(q, ldq, q_room);
+  // A tile kernel's time is its rounds over the machine times a stage's time, measured in us at
+  // K = 4096 and 8192: 64 x 64 0.55 with two blocks a CU; 128 x 128 0.8 with one, 1.1 with two (of half
+  // the stages in LDS); 256 x 256 1.8 with one.  4096^3: 73 us on the largest, 90 on 128 x 128; 512 x
+  // 4096 x 4096: 20 us on the smallest, 25 on 128 x 128.
+  const int64_t cu = device_cu_count();
+  auto rounds = [&](int t, int64_t slots) {
+    const int64_t tiles = (M + t - 1) / t * cdiv(N, t);
+    return (double)((tiles + slots - 1) / slots);
+  };
+  const double c64 = 0.55 * rounds(64, 2 * cu), c128 = 0.8 * rounds(128, cu), c128x2 = 1.1 * rounds(128, 2 * cu);
+  const double c256 = dw && dq ? 1.8 * rounds(256, cu) : 1e30;
   MX_BY_TYPE(ytype, T, {
-    if (M >= 1024 && N >= 1024) launch_gemm<T, 256, 256, 2, 4>(a, dma, st);
-    else launch_gemm<T, 128, 128, 2, 2>(a, dma, st);
+    // few tokens: the weight's bytes, at 4.5 TB/s; 32 tokens of 4096 x 4096 9 us, 19 on tiles
+    if (M <= 16 || K < 16) launch_skinny<T, 1, 1>(a, st);
+    else if (M <= 32) launch_skinny<T, 1, 2>(a, st);
+    else if (c64 <= c128 && c64 <= c128x2 && c64 <= c256) launch_gemm<T, 64, 64, 2, 2, 4>(a, dw, dq, st);
+    else if (c128 <= c128x2 && c128 <= c256 && dw && dq) launch_gemm<T, 128, 128, 2, 4, 4>(a, dw, dq, st);
+    else if (c128x2 <= c256) launch_gemm<T, 128, 128, 2, 4, 2>(a, dw, dq, st);
+    else launch_gemm<T, 256, 256, 2, 4, 2>(a, dw, dq, st);
   });
 }
 

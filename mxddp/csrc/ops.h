@@ -299,9 +299,11 @@ constexpr int64_t kInt8MaxLd = 1 << 22;  // largest row stride: a tile's rows ar
 // (at least 2^-126; NaN, with q = 0, for a row that is not finite)
 void quantize_rows(const void* x, int xtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K,
                    hipStream_t st);
-// y [M][N] = relu?((q w^T) xs[m] ws[n] + bias[n])
-void linear_int8(const int8_t* q, int64_t ldq, const float* xs, const int8_t* w, int64_t ldw, const float* ws,
-                 const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu, hipStream_t st);
+// y [M][N] = relu?((q w^T) xs[m] ws[n] + bias[n]).  room: the bytes of every row, from its start, that
+// may be read (>= K); behind K those of q hold zeros, those of w anything
+void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, const int8_t* w, int64_t ldw, int w_room,
+                 const float* ws, const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu,
+                 hipStream_t st);
 
 // ---- learning from a teacher (distill.hip) ----
 constexpr int kTopMax = 256;  // most top logits of a row

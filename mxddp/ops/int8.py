@@ -50,6 +50,15 @@ def _quantize(x2, q, ldq, scale):
                                x2.shape[0], x2.shape[1], stream_of(x2))
 
 
+def _room(w, K):
+    """Bytes that may be read of each of w's rows: whole 16-byte pieces where its memory goes on."""
+    pieces = (K + 15) // 16 * 16
+    if pieces == K:
+        return K
+    last = w.storage_offset() + (w.shape[0] - 1) * w.stride(0)
+    return pieces if last + pieces <= w.untyped_storage().nbytes() else K
+
+
 def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
                 relu: bool = False, x_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
     """``relu?((q @ weight.T) * s[..., None] * weight_scale + bias)`` for (q, s) = quantize_rows(x).
@@ -97,6 +106,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         raise ValueError(f"linear_int8: {M} rows, at most {MAX_ROWS}")
     if (weight.stride(1) != 1 and K > 1) or weight.stride(0) > _MAX_LD:
         weight = weight.contiguous()
+    weight_scale = weight_scale.contiguous()
+    bias = None if bias is None else bias.contiguous()
     y = torch.empty((*x.shape[:-1], N), device=x.device, dtype=out_dtype)
     if given:
         x2 = x2 if x2.stride(0) <= _MAX_LD else x2.contiguous()
@@ -107,7 +118,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         s = torch.empty((M,), device=x.device, dtype=torch.float32)
         _quantize(x2, q, ldq, s)
     with on_device(x2):
-        native().linear_int8(q.data_ptr(), ldq, s.data_ptr(), weight.data_ptr(), weight.stride(0),
-                             weight_scale.contiguous().data_ptr(), 0 if bias is None else bias.contiguous().data_ptr(),
-                             y.data_ptr(), DTYPES[out_dtype], M, N, K, bool(relu), stream_of(x2))
+        native().linear_int8(q.data_ptr(), ldq, K if given else ldq, s.data_ptr(), weight.data_ptr(), weight.stride(0),
+                             _room(weight, K), weight_scale.data_ptr(), _p(bias), y.data_ptr(), DTYPES[out_dtype], M,
+                             N, K, bool(relu), stream_of(x2))
     return y

@@ -257,9 +257,9 @@ def test_refusals_native(cuda):
 
     C = native()
     with pytest.raises(RuntimeError):
-        C.linear_int8(0, 16, 0, 0, 16, 0, 0, 0, 0, 4, 4, 2**17, False, 0)
+        C.linear_int8(0, 16, 16, 0, 0, 16, 16, 0, 0, 0, 0, 4, 4, 2**17, False, 0)
     with pytest.raises(RuntimeError):
-        C.linear_int8(0, 16, 0, 0, 16, 0, 0, 0, 0, 4, 0, 16, False, 0)
+        C.linear_int8(0, 16, 16, 0, 0, 16, 16, 0, 0, 0, 0, 4, 0, 16, False, 0)
     with pytest.raises(RuntimeError):
         C.quantize_rows(0, 0, 16, 0, 8, 0, 4, 16, 0)
     with pytest.raises(RuntimeError):
