@@ -282,12 +282,13 @@ PYBIND11_MODULE(_C, m) {
   m.def("distill_fwd", [](uintptr_t z, uintptr_t tv, uintptr_t ti, uintptr_t target, uintptr_t tlse, uintptr_t stats,
                           int64_t ldz, int64_t rows, int V, int k, int type, int tv_type, bool ti64, bool target64,
                           double temperature, double hard, uintptr_t loss_rows, uintptr_t loss, bool mean,
-                          uintptr_t st) {
+                          uintptr_t scratch, uintptr_t st) {
     distill_fwd(DistillArgs{P<const void>(z), P<const void>(tv), P<const void>(ti), P<const void>(target),
                             P<const float>(tlse), P<float>(stats), ldz, rows, V, k, type, tv_type, ti64, target64,
                             temperature, hard},
-                P<float>(loss_rows), P<float>(loss), mean, S(st));
+                P<float>(loss_rows), P<float>(loss), mean, P<float>(scratch), S(st));
   });
+  m.def("distill_scratch", &distill_scratch);
   m.def("distill_bwd", [](uintptr_t z, uintptr_t tv, uintptr_t ti, uintptr_t target, uintptr_t tlse, uintptr_t stats,
                           int64_t ldz, int64_t rows, int V, int k, int type, int tv_type, bool ti64, bool target64,
                           double temperature, double hard, uintptr_t dloss, bool per_row, uintptr_t dz,

@@ -367,9 +367,15 @@ __global__ __launch_bounds__(kT) void top_merge_k(TopArgs a) {
 
 // blocks of a row: long rows that alone would not fill the machine are cut into pieces of 8,192
 // classes or more, one tile of a block of 256 threads for a 16-bit type
-int top_segments(int64_t rows, int V) {
+int row_segments(int64_t rows, int V) {
   const int64_t want = (2 * device_cu_count() + rows - 1) / std::max<int64_t>(rows, 1);
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, (V + 8191) / 8192, 32}));
+}
+
+int segment_length(int V, int* nseg) {
+  const int len = *nseg == 1 ? V : (cdiv(V, *nseg) + 63) / 64 * 64;
+  *nseg = cdiv(V, len);
+  return len;
 }
 
 template <class T, int TB>
@@ -406,40 +412,54 @@ __device__ __forceinline__ void load_entry(const DistillArgs& a, int64_t row, do
   }
 }
 
-constexpr int kMaskBits = 1 << 17;  // named classes are marked in LDS, this many classes at a time
+// ---------------------------------------------------------------------------- distillation loss
+// Forward: a block takes a row, or a segment of one where there are few rows, in pieces of 16 bytes;
+// bound by the row's bytes.  Classes outside the named ones are told by a bit each in LDS, looked at
+// once a piece.  Backward: the same pieces, read again and written; the named classes and the label
+// are written over afterwards by their own threads.
+constexpr int kMaskBits = 1 << 17;  // classes whose bits are in LDS at a time
 
-template <class T>
-__global__ __launch_bounds__(kT) void distill_fwd_k(DistillArgs a, float* __restrict__ loss_rows) {
-  __shared__ float red[2 * kT / 64];
-  __shared__ double redd[kT / 64];
-  __shared__ int cls_s[kT];
-  __shared__ uint32_t mask[kMaskBits / 32];
-  const int tid = threadIdx.x;
-  const int64_t row = blockIdx.x;
-  const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
-  float* st = a.stats + row * kDistillStats;
-  const double inv_t = 1.0 / a.temperature;
-  const float c = (float)(kLog2e * inv_t), c1 = (float)kLog2e;
-  int cls;
-  double u;
-  load_entry(a, row, inv_t, &cls, &u);
-  cls_s[tid] = cls;
-  const bool any = __syncthreads_or(cls >= 0);
-  const int64_t y = a.target ? load_int(a.target, row, a.target64) : -1;
-  const bool counted = a.target ? y >= 0 && y < a.V : any;
-  if (!counted) {
-    if (tid == 0) loss_rows[row] = 0.f;
-    if (tid < kDistillStats) st[tid] = 0.f;
-    return;
+// sums of a row's exponentials at T, and at 1 where the labels need it too, relative to one maximum
+struct Sums {
+  float m = kLowest, s = 0.f, s1 = 0.f;
+  __device__ __forceinline__ void merge(float om, float os, float os1, float c, float c1) {
+    const float n = fmaxf(m, om), a = m - n, b = om - n;
+    s = s * exp2_raw(a * c) + os * exp2_raw(b * c);
+    s1 = s1 * exp2_raw(a * c1) + os1 * exp2_raw(b * c1);
+    m = n;
   }
-  bool first = cls >= 0;  // not named by an earlier entry
-  for (int j = 0; j < a.k && j < tid; ++j) first = first && cls_s[j] != cls;
-  // the classes outside (with the teacher's lse) or all of them
+};
+
+__device__ __forceinline__ Sums block_merge(Sums v, float c, float c1, float* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float om = __shfl_xor(v.m, o, 64), os = __shfl_xor(v.s, o, 64), os1 = __shfl_xor(v.s1, o, 64);
+    v.merge(om, os, os1, c, c1);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    float* r = red + 3 * (threadIdx.x >> 6);
+    r[0] = v.m;
+    r[1] = v.s;
+    r[2] = v.s1;
+  }
+  __syncthreads();
+  Sums t;
+  for (int w = 0; w < kT / 64; ++w) t.merge(red[3 * w], red[3 * w + 1], red[3 * w + 2], c, c1);
+  return t;
+}
+
+// classes [begin, end) of a row; `two`: both sums
+template <class T>
+__device__ __forceinline__ Sums row_sums(const DistillArgs& a, const typename T::store_t* z, int begin, int end,
+                                         int cls, bool two, uint32_t* mask, float* red) {
+  constexpr int N = Piece<T>::kN;
+  const int tid = threadIdx.x;
+  const float c = (float)(kLog2e / a.temperature), c1 = (float)kLog2e;
   const bool tail = a.tlse != nullptr;
-  const bool two = a.hard > 0 && a.temperature != 1.0;
-  MaxSum out, one;
-  for (int v0 = 0; v0 < a.V; v0 += kMaskBits) {
-    const int n = min(a.V - v0, kMaskBits);
+  Sums v;
+  for (int v0 = begin; v0 < end; v0 += kMaskBits) {
+    const int n = min(end - v0, kMaskBits);
     if (tail) {
       __syncthreads();
       for (int i = tid; i < (n + 31) / 32; i += kT) mask[i] = 0;
@@ -447,44 +467,113 @@ __global__ __launch_bounds__(kT) void distill_fwd_k(DistillArgs a, float* __rest
       if (cls >= v0 && cls < v0 + n) atomicOr(&mask[(cls - v0) >> 5], 1u << ((cls - v0) & 31));
       __syncthreads();
     }
-    for (int i = tid; i < n; i += kT) {
-      const float v = T::load(z[v0 + i]);
-      if (!tail || !((mask[i >> 5] >> (i & 31)) & 1)) out.add(v, c);
-      if (two) one.add(v, c1);
+    for (int base = tid * N; base < n; base += kT * kU * N) {
+      Piece<T> x[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) x[u].load(z + v0, base + u * kT * N, n, T::kNegInf);
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int i = base + u * kT * N;
+        float f[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = x[u].get(e);
+        if (tail && i < n) {
+          const uint32_t bits = mask[i >> 5] >> (i & 31);
+          if (bits & ((1u << N) - 1)) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = bits >> e & 1 ? -INFINITY : f[e];
+          }
+        }
+        float top = f[0];
+#pragma unroll
+        for (int e = 1; e < N; ++e) top = fmaxf(top, f[e]);
+        if (top > v.m) {
+          v.s *= exp2_raw((v.m - top) * c);
+          if (two) v.s1 *= exp2_raw((v.m - top) * c1);
+          v.m = top;
+        }
+        float s = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) s += exp2_raw((f[e] - v.m) * c);
+        v.s += s;
+        if (two) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) s1 += exp2_raw((f[e] - v.m) * c1);
+          v.s1 += s1;
+        }
+      }
     }
   }
-  out = block_merge<kT>(out, c, red);
-  if (two) one = block_merge<kT>(one, c1, red);
-  // all classes: those outside and the named ones, each once
-  MaxSum in;
-  const float zc = cls >= 0 ? T::load(z[cls]) : 0.f;
-  if (tail && first) in.add(zc, c);
-  in = block_merge<kT>(in, c, red);
-  MaxSum all = out;
-  if (tail) all.merge(in.m, in.s, c);
-  if (two) { one.s *= exp2f((one.m - all.m) * c1); one.m = all.m; }
+  return block_merge(v, c, c1, red);
+}
+
+struct RowShared {
+  float red[3 * kT / 64];
+  double redd[kT / 64];
+  int cls[kT];
+};
+
+// the row's named entry of this thread, the label, whether the row counts (block-wide)
+struct RowEntry {
+  int cls;
+  double u;
+  bool any, counted;
+  int64_t y;
+  __device__ __forceinline__ RowEntry(const DistillArgs& a, int64_t row, RowShared& sh) {
+    load_entry(a, row, 1.0 / a.temperature, &cls, &u);
+    sh.cls[threadIdx.x] = cls;
+    any = __syncthreads_or(cls >= 0);
+    y = a.target ? load_int(a.target, row, a.target64) : -1;
+    counted = a.target ? y >= 0 && y < a.V : any;
+  }
+};
+
+// the row's loss and what its backward needs, from the sums over the classes outside the named ones
+// (with the teacher's lse) or over all
+template <class T>
+__device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, const typename T::store_t* z,
+                                           const RowEntry& r, const Sums& out, RowShared& sh, float* loss_rows) {
+  const int tid = threadIdx.x;
+  const double inv_t = 1.0 / a.temperature;
+  const float c = (float)(kLog2e * inv_t), c1 = (float)kLog2e;
+  const bool tail = a.tlse != nullptr, two = a.hard > 0 && a.temperature != 1.0;
+  float* st = a.stats + row * kDistillStats;
+  const float zc = r.cls >= 0 ? T::load(z[r.cls]) : 0.f;
+  Sums all = out;
+  if (tail) {  // and the named ones, each class once
+    bool first = r.cls >= 0;
+    for (int j = 0; j < a.k && j < tid; ++j) first = first && sh.cls[j] != r.cls;
+    Sums in;
+    if (first && !(zc < kLowest)) {
+      in.m = zc == zc ? zc : kLowest;
+      in.s = in.s1 = zc == zc ? 1.f : zc;
+    }
+    in = block_merge(in, c, c1, sh.red);
+    all.merge(in.m, in.s, in.s1, c, c1);
+  }
   const double log_z = log((double)all.s);
   // the teacher
   double norm = 0;
-  if (tail) norm = a.tlse[row];
-  else if (any) {
-    double most = cls >= 0 ? u : -INFINITY;
+  if (tail) {
+    norm = a.tlse[row];
+  } else if (r.any) {
+    double most = r.cls >= 0 ? r.u : -INFINITY;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) most = fmax(most, __shfl_xor(most, o, 64));
     __syncthreads();
-    if ((tid & 63) == 0) redd[tid >> 6] = most;
+    if ((tid & 63) == 0) sh.redd[tid >> 6] = most;
     __syncthreads();
-    for (int w = 0; w < kT / 64; ++w) most = fmax(most, redd[w]);
-    norm = most + log(block_sum_d(cls >= 0 ? exp(u - most) : 0.0, redd));
+    for (int w = 0; w < kT / 64; ++w) most = fmax(most, sh.redd[w]);
+    norm = most + log(block_sum_d(r.cls >= 0 ? exp(r.u - most) : 0.0, sh.redd));
   }
-  const double p = cls >= 0 ? exp(u - norm) : 0.0;
+  const double p = r.cls >= 0 ? exp(r.u - norm) : 0.0;
   // p = 0 has no term, whatever the student's value
-  double kd = block_sum_d(p == 0 ? 0.0 : p * ((u - norm) - (((double)zc - all.m) * inv_t - log_z)), redd);
-  const double named = block_sum_d(p, redd);
+  double kd = block_sum_d(p == 0 ? 0.0 : p * ((r.u - norm) - (((double)zc - all.m) * inv_t - log_z)), sh.redd);
+  const double named = tail ? block_sum_d(p, sh.redd) : 1.0;
   if (tid != 0) return;
   // exp2((z - out.m) c) * co: the share of a class outside
   const bool has_out = out.s > 0.f || out.s != out.s;
-  double mass = tail ? named : any ? 1.0 : 0.0, rest = 0.0;
+  double mass = tail ? named : r.any ? 1.0 : 0.0, rest = 0.0;
   const double shift = ((double)out.m - all.m) * inv_t;
   if (tail && has_out && !(named >= 1)) {
     rest = 1.0 - named;
@@ -494,15 +583,15 @@ __global__ __launch_bounds__(kT) void distill_fwd_k(DistillArgs a, float* __rest
   const double co = has_out ? mass * exp(shift) / all.s - (tail ? rest / out.s : 0.0)
                     : all.s > 0.f ? 0.0 : __builtin_nan("");  // a row of -inf has no distribution
   const float ref = has_out ? out.m : all.m;
-  const double h = a.hard, z1 = two ? (double)one.s : (double)all.s;
+  const double h = a.hard, z1 = two ? (double)all.s1 : (double)all.s;
   double loss = (1 - h) * a.temperature * a.temperature * kd;
-  if (h > 0) loss += h * (log(z1) - ((double)T::load(z[y]) - all.m));
+  if (h > 0) loss += h * (log(z1) - ((double)T::load(z[r.y]) - all.m));
   loss_rows[row] = (float)loss;
   const double w = (1 - h) * a.temperature;
   st[0] = ref;
   st[1] = (float)(w * co + (h > 0 && !two ? h * exp((double)ref - all.m) / z1 : 0.0));
   st[2] = all.m;
-  st[3] = any ? (float)(w * mass / all.s) : 0.f;
+  st[3] = r.any ? (float)(w * mass / all.s) : 0.f;
   st[4] = h > 0 ? (float)(h / z1) : 0.f;
   st[5] = 1.f;
   const float hi = (float)norm;
@@ -510,18 +599,81 @@ __global__ __launch_bounds__(kT) void distill_fwd_k(DistillArgs a, float* __rest
   st[7] = (float)(norm - hi);
 }
 
+__device__ __forceinline__ void leave_out(const DistillArgs& a, int64_t row, float* loss_rows) {
+  if (threadIdx.x == 0) loss_rows[row] = 0.f;
+  if (threadIdx.x < kDistillStats) a.stats[row * kDistillStats + threadIdx.x] = 0.f;
+}
+
+// part == nullptr: a block has the whole row; else [rows][nseg] sums of a segment each, for distill_join_k
+template <class T>
+__global__ __launch_bounds__(kT) void distill_fwd_k(DistillArgs a, int nseg, int seglen, float* __restrict__ part,
+                                                    float* __restrict__ loss_rows) {
+  __shared__ RowShared sh;
+  __shared__ uint32_t mask[kMaskBits / 32];
+  const int64_t row = blockIdx.x / nseg;
+  const int seg = blockIdx.x % nseg;
+  const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
+  const RowEntry r(a, row, sh);
+  if (!r.counted) {
+    if (!part) leave_out(a, row, loss_rows);
+    return;
+  }
+  const bool two = a.hard > 0 && a.temperature != 1.0;
+  const Sums out = row_sums<T>(a, z, seg * seglen, min(a.V, (seg + 1) * seglen), r.cls, two, mask, sh.red);
+  if (!part) {
+    finish_row<T>(a, row, z, r, out, sh, loss_rows);
+  } else if (threadIdx.x == 0) {
+    float* p = part + (row * nseg + seg) * 3;
+    p[0] = out.m;
+    p[1] = out.s;
+    p[2] = out.s1;
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(kT) void distill_join_k(DistillArgs a, int nseg, const float* __restrict__ part,
+                                                     float* __restrict__ loss_rows) {
+  __shared__ RowShared sh;
+  const int64_t row = blockIdx.x;
+  const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
+  const RowEntry r(a, row, sh);
+  if (!r.counted) return leave_out(a, row, loss_rows);
+  Sums v;
+  if ((int)threadIdx.x < nseg) {
+    const float* p = part + (row * nseg + threadIdx.x) * 3;
+    v.m = p[0];
+    v.s = p[1];
+    v.s1 = p[2];
+  }
+  v = block_merge(v, (float)(kLog2e / a.temperature), (float)kLog2e, sh.red);
+  finish_row<T>(a, row, z, r, v, sh, loss_rows);
+}
+
 // loss = the sum or mean of the rows' losses; the rows' weight goes behind their statistics
-__global__ __launch_bounds__(kT) void distill_mean_k(const float* __restrict__ loss_rows, float* __restrict__ stats,
-                                                     int64_t rows, int mean, float* __restrict__ loss) {
-  __shared__ double red[kT / 64];
+__global__ __launch_bounds__(1024) void distill_mean_k(const float* __restrict__ loss_rows, float* __restrict__ stats,
+                                                       int64_t rows, int mean, float* __restrict__ loss) {
+  __shared__ double red[2][16];
   double s = 0, n = 0;
-  for (int64_t i = threadIdx.x; i < rows; i += kT) {
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) {
     s += loss_rows[i];
     n += stats[i * kDistillStats + 5];
   }
-  s = block_sum_d(s, red);
-  n = block_sum_d(n, red);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o, 64);
+    n += __shfl_xor(n, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    red[0][threadIdx.x >> 6] = s;
+    red[1][threadIdx.x >> 6] = n;
+  }
+  __syncthreads();
   if (threadIdx.x == 0) {
+    s = n = 0;
+    for (int w = 0; w < 16; ++w) {
+      s += red[0][w];
+      n += red[1][w];
+    }
     const double inv = mean ? 1.0 / fmax(n, 1.0) : 1.0;
     *loss = (float)(s * inv);
     stats[rows * kDistillStats] = (float)inv;
@@ -529,17 +681,25 @@ __global__ __launch_bounds__(kT) void distill_mean_k(const float* __restrict__ l
 }
 
 template <class T>
-__global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, const float* __restrict__ dloss, int per_row,
+__global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int seglen,
+                                                    const float* __restrict__ dloss, int per_row,
                                                     typename T::store_t* __restrict__ dz) {
+  constexpr int N = Piece<T>::kN;
   __shared__ int cls_s[kT];
   __shared__ float p_s[kT];
   const int tid = threadIdx.x;
-  const int64_t row = blockIdx.x;
+  const int64_t row = blockIdx.x / nseg;
+  const int begin = (int)(blockIdx.x % nseg) * seglen, end = min(a.V, begin + seglen);
   const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
   const float* st = a.stats + row * kDistillStats;
   dz += row * a.V;
-  if (st[5] == 0.f) {
-    for (int i = tid; i < a.V; i += kT) dz[i] = T::store(0.f);
+  if (st[5] == 0.f) {  // a row that is left out: its logits are not looked at
+    const Bytes16 zero = {{0, 0, 0, 0}};
+    for (int i = begin + tid * N; i < end; i += kT * N) {
+      if (i + N <= end) *reinterpret_cast<Bytes16*>(dz + i) = zero;
+      else
+        for (int e = i; e < end; ++e) dz[e] = 0;
+    }
     return;
   }
   const float g = per_row ? dloss[row] : *dloss * a.stats[a.rows * kDistillStats];
@@ -547,11 +707,31 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, const float* 
   const float c = (float)(kLog2e * inv_t), c1 = (float)kLog2e;
   const bool two = a.hard > 0 && a.temperature != 1.0;
   const float ref = st[0], co = st[1], m = st[2], ci = st[3], h1 = st[4];
-  for (int i = tid; i < a.V; i += kT) {
-    const float v = T::load(z[i]);
-    float d = co == 0.f ? 0.f : co * exp2f((v - ref) * c);
-    if (two) d += h1 * exp2f((v - m) * c1);
-    dz[i] = T::store(g * d);
+  // without a share (co = 0) a named class above `ref` must not make a NaN of an overflow
+  const float lim = co == 0.f ? 0.f : INFINITY;
+  for (int base = begin + tid * N; base < end; base += kT * kU * N) {
+    Piece<T> x[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) x[u].load(z, base + u * kT * N, end, T::kNegInf);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int i = base + u * kT * N;
+      typename T::store_t o[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float v = x[u].get(e);
+        float d = co * fminf(exp2_raw((v - ref) * c), lim);
+        if (two) d += h1 * exp2_raw((v - m) * c1);
+        o[e] = T::store(g * d);
+      }
+      if (i + N <= end) {
+        __builtin_memcpy(dz + i, o, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (i + e < end) dz[i + e] = o[e];
+      }
+    }
   }
   int cls;
   double u;
@@ -560,24 +740,21 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, const float* 
   p_s[tid] = cls >= 0 ? (float)((1 - a.hard) * a.temperature * exp(u - st[6] - st[7])) : 0.f;
   const int64_t y = a.hard > 0 ? load_int(a.target, row, a.target64) : -1;
   __syncthreads();  // also orders the stores above before the ones below
-  auto put = [&](int i, float p, bool is_y) {
-    const float v = T::load(z[i]);
-    const float q = ci == 0.f ? 0.f : ci * exp2f((v - m) * c);
-    float d = q - p;
-    if (a.hard > 0) d += h1 * exp2f((v - m) * c1) - (is_y ? (float)a.hard : 0.f);
-    dz[i] = T::store(g * d);
-  };
-  if (cls >= 0) {
+  if (cls >= begin && cls < end) {
     float p = 0;  // a class that is named twice has both entries' share
     for (int j = 0; j < a.k; ++j) p += cls_s[j] == cls ? p_s[j] : 0.f;
-    put(cls, p, cls == y);
+    const float v = T::load(z[cls]);
+    const float q = ci == 0.f ? 0.f : ci * exp2f((v - m) * c);
+    float d = q - p;
+    if (a.hard > 0) d += h1 * exp2f((v - m) * c1) - (cls == y ? (float)a.hard : 0.f);
+    dz[cls] = T::store(g * d);
   }
-  if (tid == 0 && y >= 0) {
+  if (tid == 0 && y >= begin && y < end) {
     bool named = false;
     for (int j = 0; j < a.k; ++j) named = named || cls_s[j] == y;
     if (!named) {
       const float v = T::load(z[y]);
-      float d = co == 0.f ? 0.f : co * exp2f((v - ref) * c);
+      float d = co * fminf(exp2f((v - ref) * c), lim);
       if (two) d += h1 * exp2f((v - m) * c1);
       dz[y] = T::store(g * (d - (float)a.hard));
     }
@@ -585,7 +762,7 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, const float* 
 }
 
 void check_distill(const DistillArgs& a) {
-  MX_CHECK(a.rows >= 0 && a.rows < (1ll << 31) && a.V >= 1 && a.V <= (1 << 30) && a.k >= 1 && a.k <= kTopMax,
+  MX_CHECK(a.rows >= 0 && a.rows <= kMaxRows && a.V >= 1 && a.V <= (1 << 30) && a.k >= 1 && a.k <= kTopMax,
            "distill_loss: bad sizes");
   MX_CHECK(a.temperature > 0 && a.hard >= 0 && a.hard <= 1 && (a.hard == 0 || a.target), "distill_loss: bad weights");
 }
@@ -593,23 +770,20 @@ void check_distill(const DistillArgs& a) {
 }  // namespace
 
 int64_t top_logits_scratch(int64_t rows, int V, int k) {
-  const int nseg = top_segments(rows, V);
+  const int nseg = row_segments(rows, V);
   return nseg > 1 ? rows * nseg * (k + 1) : 0;
 }
 
 void top_logits(const void* z, int type, int64_t ldz, int64_t rows, int V, int k, double temperature, void* values,
                 int32_t* index, float* lse, void* scratch, hipStream_t st) {
-  MX_CHECK(rows >= 0 && rows < (1ll << 31) && V >= 1 && V <= (1 << 30) && k >= 1 && k <= kTopMax && k <= V &&
+  MX_CHECK(rows >= 0 && rows <= kMaxRows && V >= 1 && V <= (1 << 30) && k >= 1 && k <= kTopMax && k <= V &&
                temperature > 0,
            "top_logits: bad sizes");
   if (rows == 0) return;
-  TopArgs a{z, values, index, lse, static_cast<uint64_t*>(scratch), ldz, rows, V, k, top_segments(rows, V), V,
+  TopArgs a{z, values, index, lse, static_cast<uint64_t*>(scratch), ldz, rows, V, k, row_segments(rows, V), V,
             (float)(kLog2e / temperature), (float)(1.0 / temperature)};
-  if (a.nseg > 1) {
-    MX_CHECK(scratch, "top_logits: long rows need scratch");
-    a.seglen = (cdiv(V, a.nseg) + 63) / 64 * 64;
-    a.nseg = cdiv(V, a.seglen);
-  }
+  a.seglen = segment_length(V, &a.nseg);
+  MX_CHECK(a.nseg == 1 || scratch, "top_logits: long rows need scratch");
   // one tile where a block's part of the row fits: a wave alone needs no barrier
   MX_BY_TYPE(type, T, {
     constexpr int wave_tile = 64 * kU * Piece<T>::kN;
@@ -620,18 +794,33 @@ void top_logits(const void* z, int type, int64_t ldz, int64_t rows, int V, int k
   });
 }
 
-void distill_fwd(const DistillArgs& a, float* loss_rows, float* loss, bool mean, hipStream_t st) {
+int64_t distill_scratch(int64_t rows, int V) {
+  const int nseg = row_segments(rows, V);
+  return nseg > 1 ? 3 * rows * nseg : 0;
+}
+
+void distill_fwd(const DistillArgs& a, float* loss_rows, float* loss, bool mean, float* scratch, hipStream_t st) {
   check_distill(a);
+  int nseg = row_segments(a.rows, a.V);
+  const int seglen = segment_length(a.V, &nseg);
+  MX_CHECK(nseg == 1 || scratch, "distill_loss: long rows need scratch");
   if (a.rows > 0)
-    MX_BY_TYPE(a.type, T, MX_LAUNCH(distill_fwd_k<T>, dim3((uint32_t)a.rows), dim3(kT), 0, st, a, loss_rows));
-  if (loss) MX_LAUNCH(distill_mean_k, dim3(1), dim3(kT), 0, st, loss_rows, a.stats, a.rows, mean ? 1 : 0, loss);
+    MX_BY_TYPE(a.type, T, {
+      MX_LAUNCH(distill_fwd_k<T>, dim3((uint32_t)(a.rows * nseg)), dim3(kT), 0, st, a, nseg, seglen,
+                nseg > 1 ? scratch : nullptr, loss_rows);
+      if (nseg > 1)
+        MX_LAUNCH(distill_join_k<T>, dim3((uint32_t)a.rows), dim3(kT), 0, st, a, nseg, scratch, loss_rows);
+    });
+  if (loss) MX_LAUNCH(distill_mean_k, dim3(1), dim3(1024), 0, st, loss_rows, a.stats, a.rows, mean ? 1 : 0, loss);
 }
 
 void distill_bwd(const DistillArgs& a, const float* dloss, bool per_row, void* dz, hipStream_t st) {
   check_distill(a);
+  int nseg = row_segments(a.rows, a.V);
+  const int seglen = segment_length(a.V, &nseg);
   if (a.rows > 0)
-    MX_BY_TYPE(a.type, T, MX_LAUNCH(distill_bwd_k<T>, dim3((uint32_t)a.rows), dim3(kT), 0, st, a, dloss,
-                                    per_row ? 1 : 0, static_cast<typename T::store_t*>(dz)));
+    MX_BY_TYPE(a.type, T, MX_LAUNCH(distill_bwd_k<T>, dim3((uint32_t)(a.rows * nseg)), dim3(kT), 0, st, a, nseg,
+                                    seglen, dloss, per_row ? 1 : 0, static_cast<typename T::store_t*>(dz)));
 }
 
 }  // namespace mx

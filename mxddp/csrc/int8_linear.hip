@@ -334,7 +334,7 @@ template <class T, int TM, int TN, int WM, int WN, int NS>
 void launch_gemm(GemmArgs a, bool dw, bool dq, hipStream_t st) {
   a.tiles_n = cdiv(a.N, TM);
   const int64_t tm = (a.M + TN - 1) / TN;
-  MX_CHECK(tm * a.tiles_n < (1ll << 31) / 8, "linear_int8: too many tiles");
+  MX_CHECK(tm * a.tiles_n <= kMaxRows, "linear_int8: too many tiles");
   a.tiles_m = (int)tm;
   const dim3 grid((uint32_t)(tm * a.tiles_n)), block(64 * WM * WN);
   if (dw && dq) MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, NS, true, true>), grid, block, 0, st, a);
@@ -415,7 +415,7 @@ template <class T, int FM, int FN>
 void launch_skinny(GemmArgs a, hipStream_t st) {
   a.tiles_n = cdiv(a.N, 16 * FM);
   const int64_t blocks = (a.M + 16 * FN - 1) / (16 * FN) * a.tiles_n;
-  MX_CHECK(blocks < (1ll << 31), "linear_int8: too many tiles");
+  MX_CHECK(blocks <= kMaxRows, "linear_int8: too many tiles");
   MX_LAUNCH((int8_skinny_k<T, FM, FN>), dim3((uint32_t)blocks), dim3(64 * kSkinnyWaves), 0, st, a);
 }
 
@@ -423,7 +423,7 @@ void launch_skinny(GemmArgs a, hipStream_t st) {
 
 void quantize_rows(const void* x, int xtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K,
                    hipStream_t st) {
-  MX_CHECK(rows >= 0 && rows < (1ll << 31) && K >= 1 && ldq >= K, "quantize_rows: bad sizes");
+  MX_CHECK(rows >= 0 && rows <= kMaxRows && K >= 1 && ldq >= K, "quantize_rows: bad sizes");
   if (rows == 0) return;
   // one wave where a row fits its registers: no barrier
   MX_BY_TYPE(xtype, T, {
@@ -439,7 +439,7 @@ void quantize_rows(const void* x, int xtype, int64_t ldx, int8_t* q, int64_t ldq
 void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, const int8_t* w, int64_t ldw, int w_room,
                  const float* ws, const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu,
                  hipStream_t st) {
-  MX_CHECK(M >= 0 && N >= 1 && K >= 1 && K <= kInt8MaxK, "linear_int8: bad sizes");
+  MX_CHECK(M >= 0 && M <= kMaxRows && N >= 1 && K >= 1 && K <= kInt8MaxK, "linear_int8: bad sizes");
   MX_CHECK(ldq >= 0 && ldq <= kInt8MaxLd && ldw >= 0 && ldw <= kInt8MaxLd, "linear_int8: row stride too large");
   if (M == 0) return;
   GemmArgs a{q, w, xs, ws, bias, y, ldq, ldw, M, N, K, relu ? 1 : 0, 0, 0};

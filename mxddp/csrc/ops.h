@@ -291,6 +291,9 @@ void synth_templates(float* templates, int C, int D, uint64_t seed, hipStream_t 
 void augment_crop_flip_norm(const float* x, float* y, int N, int C, int H, int W, int pad,
                             const float* mean, const float* std, uint64_t seed, int32_t* counter,
                             hipStream_t st);
+// most rows (blocks of up to 512 threads) that one launch of the following takes: 2^32 threads
+constexpr int64_t kMaxRows = (1 << 23) - 1;
+
 // ---- linear layers in 8-bit integers (int8_linear.hip); element types: lowp.h DType ----
 // |q w| <= 2^14, so up to this many products sum to less than 2^31
 constexpr int kInt8MaxK = (1 << 17) - 1;
@@ -326,7 +329,9 @@ struct DistillArgs {
 };
 constexpr int kDistillStats = 8;
 // loss_rows [rows]: each row's loss; loss (or null): their mean over the counted rows, or their sum
-void distill_fwd(const DistillArgs& a, float* loss_rows, float* loss, bool mean, hipStream_t st);
+// scratch: distill_scratch(...) floats (0: none needed)
+int64_t distill_scratch(int64_t rows, int V);
+void distill_fwd(const DistillArgs& a, float* loss_rows, float* loss, bool mean, float* scratch, hipStream_t st);
 // dz [rows][V] = dloss * d loss / dz; dloss: one value, or per_row one for each row's loss
 void distill_bwd(const DistillArgs& a, const float* dloss, bool per_row, void* dz, hipStream_t st);
 

@@ -83,8 +83,11 @@ class _DistillLoss(torch.autograd.Function):
         loss_rows = torch.empty((rows,), device=z.device, dtype=torch.float32)
         loss = torch.empty((), device=z.device, dtype=torch.float32) if reduction != "none" else None
         with on_device(z):
-            native().distill_fwd(*_args(z, tv, ti, target, tlse, stats, temperature, hard), loss_rows.data_ptr(),
-                                 _p(loss), reduction == "mean", stream_of(z))
+            C = native()
+            n = C.distill_scratch(rows, z.shape[1])
+            scratch = torch.empty((n,), device=z.device, dtype=torch.float32) if n else None
+            C.distill_fwd(*_args(z, tv, ti, target, tlse, stats, temperature, hard), loss_rows.data_ptr(), _p(loss),
+                          reduction == "mean", _p(scratch), stream_of(z))
         ctx.save_for_backward(z, tv, ti, target, tlse, stats)
         ctx.args = (temperature, hard)
         ctx.per_row = loss is None

@@ -6,7 +6,7 @@ import contextlib
 import torch
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # csrc/lowp.h DType
-MAX_ROWS = 2**31 - 1
+MAX_ROWS = 2**23 - 1  # csrc/ops.h kMaxRows
 
 
 def check_float(t: torch.Tensor, name: str, cpu_double: bool = False) -> None:

@@ -183,7 +183,10 @@ def oracle(z, tv, ti, target, tlse, T, h):
             eg[y] += 4 * E * h
             tl[r] += h * es(V)
         tl[r] += 2 * E * loss[r].abs()
-        grad[r], tg[r] = g, eg + 4 * E * g.abs()
+        # the exponential of a far class is 0 below 2^-126; it is multiplied by at most w (1 / Z + rest /
+        # Z_out) + h / Z_1 with all three sums >= 1 (each holds its own maximum), so by 2 w + h
+        tg[r] = eg + 4 * E * g.abs() + 2.0**-126 * (2 * w + h)
+        grad[r] = g
     return loss, counted, grad, tl, tg
 
 
@@ -457,7 +460,7 @@ def test_refusals_native(cuda):
     with pytest.raises(RuntimeError):
         C.top_logits(0, 5, 8, 2, 8, 2, 1.0, 0, 0, 0, 0, 0)
     with pytest.raises(RuntimeError):
-        C.distill_fwd(0, 0, 0, 0, 0, 0, 8, 2, 8, 300, 0, 0, False, False, 1.0, 0.0, 0, 0, True, 0)
+        C.distill_fwd(0, 0, 0, 0, 0, 0, 8, 2, 8, 300, 0, 0, False, False, 1.0, 0.0, 0, 0, True, 0, 0)
     with pytest.raises(RuntimeError):
         C.distill_bwd(0, 0, 0, 0, 0, 0, 8, 2, 8, 3, 0, 0, False, False, 1.0, 0.5, 0, False, 0, 0)
     z, tv, ti, y, lse = make(4, 30, 3, torch.float32)
