@@ -80,20 +80,24 @@ __device__ __forceinline__ MaxSum block_merge(MaxSum v, float c, float* red) {
 }
 
 // ---------------------------------------------------------------------------- top logits
-// One pass over the row: a block of TB threads takes tiles of TB x kU pieces into registers, and of
-// each piece the maximum and the exponentials' sum.  In the first tile the threshold is the largest
-// 16-bit prefix of a value that at least k pieces' maxima reach, so at least k elements do, and for
-// independent values hardly more.  Elements that reach it become candidates in LDS; in later tiles an
-// element has to be above the threshold: one equal to it comes after k others that are as large.
-// When the list grows, its threshold is raised in the same way; where ties overflow it (constant or
-// sorted rows) the k largest keys of list and tile are selected exactly, bit by bit.  In the end a
-// candidate's place is the number of larger keys.
+// One pass over the row: a block of TB threads takes tiles of TB x kU pieces of 16 bytes into
+// registers, and of each piece the maximum and the exponentials' sum.  In the first tile the threshold
+// is the largest 16-bit prefix of a value that at least k pieces' maxima reach, so at least k elements
+// do, and for independent values hardly more.  A piece that reaches it is noted; in later tiles its
+// maximum has to be above the threshold: an equal element comes after k others that are as large.
+// When pieces have gathered, their elements become candidates in LDS and the threshold is raised to
+// what k of the candidates reach; so a row of V independent values has about k log(V / tile) noted
+// pieces.  Where ties overflow the candidates (constant or sorted rows) the k largest keys are selected
+// exactly, bit by bit.  In the end a candidate's place is the number of larger keys.
+// Bound by the row's bytes; what is done for a noted piece would otherwise be done by a whole wave.
 //
 // Few long rows are split over blocks: each leaves its segment's k largest keys, in order, and its
 // sum, and top_merge_k joins them.
-constexpr int kU = 4;       // pieces of 16 bytes a thread holds
+constexpr int kU = 4;  // pieces a thread holds
 // candidates: twice the largest k and more; a block of one wave has short rows, and many to a CU
 constexpr int top_cap(int tb) { return tb == 64 ? 512 : 1024; }
+// noted pieces: up to 2 k or 128 stay noted before a tile that may add all of its own
+constexpr int top_pieces(int tb) { return 2 * kTopMax + tb * kU; }
 
 struct TopArgs {
   const void* z;
@@ -125,16 +129,15 @@ __device__ __forceinline__ float from_order_bits(uint32_t b) {
   return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
-// The k largest of the n keys in `from` and of a tile's elements, [base, end) of z, go to `to`, in any
-// order; returns the smallest of them.  There must be k.  The tile is read again for every bit (from
-// the caches): taking it in registers would put every tile's registers in memory for this rare call.
+// The k largest of the n keys in `from` and of the elements of np noted pieces go to `to`, in any
+// order; returns the smallest of them.  There must be k.  Exact: the key is found bit by bit; the
+// pieces are read again for every bit, from the caches.
 template <class T, int TB>
 __device__ __noinline__ uint64_t select_exact(const uint64_t* from, int n, uint64_t* to,
-                                              const typename T::store_t* z, int base, int end, int k, int* slots,
-                                              int* cnt) {
+                                              const typename T::store_t* z, const int* piece, int np, int end, int k,
+                                              int* slots, int* cnt) {
   const int tid = threadIdx.x;
   constexpr int N = Piece<T>::kN;
-  const int pieces = (max(end - base, 0) + N - 1) / N;
   uint64_t t = 0;
   __syncthreads();
 #pragma unroll 1
@@ -142,8 +145,8 @@ __device__ __noinline__ uint64_t select_exact(const uint64_t* from, int n, uint6
     const uint64_t trial = t | 1ull << bit;
     int c = 0;
     for (int i = tid; i < (n + 63) / 64 * 64; i += TB) c += wave_count(i < n && from[i] >= trial);
-    for (int p = tid; p < (pieces + 63) / 64 * 64; p += TB) {
-      const int i = base + p * N;
+    for (int p = tid; p < (np + 63) / 64 * 64; p += TB) {
+      const int i = p < np ? piece[p] : end;
       Piece<T> x;
       x.load(z, i, end, T::kNegInf);
 #pragma unroll
@@ -155,15 +158,16 @@ __device__ __noinline__ uint64_t select_exact(const uint64_t* from, int n, uint6
   __syncthreads();
   for (int i = tid; i < n; i += TB)
     if (from[i] >= t) to[atomicAdd(cnt, 1)] = from[i];
-  for (int i = base + tid; i < end; i += TB) {
-    const uint64_t key = order_key(T::load(z[i]), i);
-    if (key >= t) to[atomicAdd(cnt, 1)] = key;
-  }
+  for (int p = tid; p < np; p += TB)
+    for (int i = piece[p], e = 0; e < N && i + e < end; ++e) {
+      const uint64_t key = order_key(T::load(z[i + e]), i + e);
+      if (key >= t) to[atomicAdd(cnt, 1)] = key;
+    }
   __syncthreads();
   return t;
 }
 
-// Candidates in LDS: two lists, the current one, its length, and what a further element has to exceed
+// Candidates in LDS: two lists, the current one and its length, and the threshold
 template <int TB>
 struct Candidates {
   uint64_t* list;
@@ -171,7 +175,8 @@ struct Candidates {
   int* slots;
   int* cnt;
   int n;
-  float t;
+  float t;             // a further element has to be above it
+  uint32_t floor = 0;  // its order bits
 
   // keep those that reach the largest 16-bit prefix that k of them reach
   __device__ __forceinline__ void raise(int k) {
@@ -191,7 +196,8 @@ struct Candidates {
     __syncthreads();
     n = *cnt;
     swap();
-    t = from_order_bits(prefix << 16);
+    floor = prefix << 16;
+    t = from_order_bits(floor);
   }
   __device__ __forceinline__ void swap() {
     uint64_t* l = list;
@@ -218,15 +224,17 @@ __global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
   constexpr int N = Piece<T>::kN, TILE = TB * kU * N, kCap = top_cap(TB);
   static_assert(kCap >= 2 * kTopMax, "a list that was cut to k leaves half of its room");
   __shared__ uint64_t buf[2][kCap];
-  __shared__ int slots[2 * TB / 64], cnt;
+  __shared__ int piece[top_pieces(TB)];
+  __shared__ int slots[2 * TB / 64], cnt, noted;
   __shared__ float red[2 * TB / 64];
   const int tid = threadIdx.x, k = a.k;
   const int64_t row = blockIdx.x / a.nseg;
   const int seg = blockIdx.x % a.nseg, begin = seg * a.seglen, end = min(a.V, begin + a.seglen);
   const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
+  const int gather = max(2 * k, 128);
   Candidates<TB> cand{buf[0], buf[1], slots, &cnt, 0, 0.f};
   MaxSum ms;
-  if (tid == 0) cnt = 0;
+  if (tid == 0) cnt = noted = 0;
 #pragma unroll 1
   for (int base = begin; base < end; base += TILE) {
     Piece<T> x[kU];
@@ -247,58 +255,73 @@ __global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
       odd[u] = s != s;
       ms.s += s;
     }
-    const bool first = base == begin;
-    uint32_t prefix = 0;
-    if (first) {
+    // the largest prefix that k of the tile's maxima reach (a piece of NaN alone counts as one)
+    auto tile_prefix = [&] {
+      uint32_t prefix = 0;
 #pragma unroll 1
       for (int bit = 15; bit >= 0; --bit) {
         const uint32_t trial = prefix | 1u << bit;
         int c = 0;
 #pragma unroll
-        for (int u = 0; u < kU; ++u)  // a piece of NaN alone counts as one
+        for (int u = 0; u < kU; ++u)
           c += wave_count(base + (u * TB + tid) * N < end && order_bits(top[u]) >> 16 >= trial);
         if (block_count<TB>(c, slots, bit) >= k) prefix = trial;
       }
-      cand.t = from_order_bits(prefix << 16);
+      return prefix << 16;
+    };
+    const bool first = base == begin;
+    const int before = noted;
+    if (first) {
+      cand.floor = tile_prefix();
+      cand.t = from_order_bits(cand.floor);
     }
-    __syncthreads();
+    __syncthreads();  // every thread has `before`
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int i0 = base + (u * TB + tid) * N;
-      if (odd[u] || (first ? order_bits(top[u]) >= prefix << 16 : top[u] > cand.t)) {
+      if (i0 < end && (odd[u] || (first ? order_bits(top[u]) >= cand.floor : top[u] > cand.t)))
+        piece[atomicAdd(&noted, 1)] = i0;
+    }
+    __syncthreads();
+    const int np = noted;
+    __syncthreads();  // every thread has it: what follows is block-uniform
+    const bool last = base + TILE >= end;
+    if (np > gather || last) {
+      // most of the tile above the threshold: a row that rises.  The tile has a threshold of its own.
+      if (!first && np - before > TB * kU / 2) cand.floor = max(cand.floor, tile_prefix());
+      for (int p = tid; p < np; p += TB) {
+        const int i0 = piece[p];
+        Piece<T> y;
+        y.load(z, i0, end, T::kNegInf);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          const float v = x[u].get(e);
-          if (i0 + e < end && (first ? order_bits(v) >= prefix << 16 : !(v <= cand.t))) {
+          const float v = y.get(e);
+          if (i0 + e < end && order_bits(v) >= cand.floor) {
             const int pos = atomicAdd(&cnt, 1);
             if (pos < kCap) cand.list[pos] = order_key(v, i0 + e);
           }
         }
       }
-    }
-    __syncthreads();
-    const int had = cand.n;
-    cand.n = cnt;
-    if (cand.n > kCap) {  // the exact k of the list before this tile and of the tile
-      const uint64_t low =
-          select_exact<T, TB>(cand.list, had, cand.other, z, base, min(end, base + TILE), k, slots, &cnt);
-      cand.t = from_order_bits((uint32_t)(low >> 32));
-      cand.swap();
-      cand.n = k;
-    } else if (cand.n > kCap / 2) {
-      __syncthreads();  // every thread has read cnt
-      cand.raise(k);
-      if (cand.n > kCap / 2) {
-        const uint64_t low = select_exact<T, TB>(cand.list, cand.n, cand.other, z, 0, 0, k, slots, &cnt);
-        cand.t = from_order_bits((uint32_t)(low >> 32));
+      __syncthreads();
+      const int had = cand.n;
+      cand.n = cnt;
+      __syncthreads();  // every thread has read both counters
+      cand.t = from_order_bits(cand.floor);
+      if (cand.n <= kCap && cand.n > k + 16) cand.raise(k);
+      if (cand.n > (last ? kCap : kCap / 2)) {
+        const bool over = cand.n > kCap;  // the list is what it was before, the rest is in the pieces
+        const uint64_t low = select_exact<T, TB>(cand.list, over ? had : cand.n, cand.other, z, piece, over ? np : 0,
+                                                 end, k, slots, &cnt);
+        cand.floor = (uint32_t)(low >> 32);
+        cand.t = from_order_bits(cand.floor);
         cand.swap();
         cand.n = k;
       }
+      if (tid == 0) noted = 0;
+      __syncthreads();
     }
-    __syncthreads();
   }
   ms = block_merge<TB>(ms, a.c, red);
-  if (cand.n > k + 64) cand.raise(k);
   const int n = cand.n, kk = min(k, n);
   for (int i = tid; i < n; i += TB) {
     const uint64_t key = cand.list[i];
@@ -352,7 +375,7 @@ __global__ __launch_bounds__(kT) void top_merge_k(TopArgs a) {
   cand.n = cnt;
   __syncthreads();
   if (cand.n > kCap) {
-    select_exact<T, kT>(keys, total, cand.list, z, 0, 0, k, slots, &cnt);
+    select_exact<T, kT>(keys, total, cand.list, z, nullptr, 0, 0, k, slots, &cnt);
     cand.n = k;
   } else if (cand.n > k + 64) {
     cand.raise(k);
@@ -788,8 +811,7 @@ void top_logits(const void* z, int type, int64_t ldz, int64_t rows, int V, int k
   MX_BY_TYPE(type, T, {
     constexpr int wave_tile = 64 * kU * Piece<T>::kN;
     if (a.seglen <= wave_tile) launch_top<T, 64>(a, st);
-    else if (a.seglen <= 4 * wave_tile) launch_top<T, 256>(a, st);
-    else launch_top<T, 512>(a, st);
+    else launch_top<T, 256>(a, st);
     if (a.nseg > 1) MX_LAUNCH(top_merge_k<T>, dim3((uint32_t)rows), dim3(kT), 0, st, a);
   });
 }
