@@ -273,6 +273,13 @@ PYBIND11_MODULE(_C, m) {
     linear_int8(P<const int8_t>(q), ldq, q_room, P<const float>(xs), P<const int8_t>(w), ldw, w_room,
                 P<const float>(ws), P<const float>(bias), P<void>(y), ytype, M, N, K, relu, S(st));
   });
+  m.def("linear_int8_scratch", &linear_int8_scratch);
+  m.def("linear_int8_float", [](uintptr_t x, int xtype, int64_t ldx, uintptr_t w, int64_t ldw, int w_room, uintptr_t ws,
+                                uintptr_t bias, uintptr_t y, int ytype, int64_t M, int N, int K, bool relu,
+                                uintptr_t scratch, uintptr_t st) {
+    linear_int8_float(P<const void>(x), xtype, ldx, P<const int8_t>(w), ldw, w_room, P<const float>(ws),
+                      P<const float>(bias), P<void>(y), ytype, M, N, K, relu, P<void>(scratch), S(st));
+  });
   m.def("top_logits", [](uintptr_t z, int type, int64_t ldz, int64_t rows, int V, int k, double temperature,
                          uintptr_t values, uintptr_t index, uintptr_t lse, uintptr_t scratch, uintptr_t st) {
     top_logits(P<const void>(z), type, ldz, rows, V, k, temperature, P<void>(values), P<int32_t>(index),

@@ -27,6 +27,40 @@ __device__ __forceinline__ int quant1(float x, float s, float inv) {
   return (int)q;
 }
 
+// A row's scale from its largest magnitude's bits (a thread's in, the block's out).  Infinities and NaN
+// are above every number.
+struct RowScale {
+  float s, inv;
+  bool ok;
+};
+template <int TB>
+__device__ __forceinline__ RowScale row_scale(uint32_t top, uint32_t* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+  if constexpr (TB > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TB / 64; ++w) top = max(top, red[w]);
+  }
+  RowScale r;
+  r.ok = top < 0x7f800000u;
+  r.s = r.ok ? fmaxf(__uint_as_float(top) / 127.f, kTiny) : __builtin_nanf("");
+  r.inv = 1.f / r.s;
+  return r;
+}
+
+template <class T>
+__device__ __forceinline__ void quant_piece(const Piece<T>& p, const RowScale& sc, uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < Piece<T>::kN / 4; ++i) {
+    w[i] = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[i] |= (uint32_t)((sc.ok ? quant1(p.get(4 * i + e), sc.s, sc.inv) : 0) & 0xff) << (8 * e);
+  }
+}
+
 // One row a block of TB threads.  Bound by its bytes: up to kQP pieces of 16 bytes a thread stay in
 // registers between the maximum and the rounding; a longer row is read again, from the cache.
 constexpr int kQP = 4;
@@ -42,7 +76,6 @@ __global__ __launch_bounds__(TB) void quantize_rows_k(const typename T::store_t*
   x += row * ldx;
   q += row * ldq;
   Piece<T> p[kQP];
-  // the largest magnitude as bits: infinities and NaN are above every number
   uint32_t top = 0;
   for (int k0 = 0; k0 < K; k0 += TILE) {
 #pragma unroll
@@ -52,31 +85,15 @@ __global__ __launch_bounds__(TB) void quantize_rows_k(const typename T::store_t*
 #pragma unroll
       for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(p[u].get(e)) & 0x7fffffffu);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-  if constexpr (TB > 64) {
-    if ((tid & 63) == 0) red[tid >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < TB / 64; ++w) top = max(top, red[w]);
-  }
-  const bool ok = top < 0x7f800000u;
-  const float s = ok ? fmaxf(__uint_as_float(top) / 127.f, kTiny) : __builtin_nanf("");
-  const float inv = 1.f / s;
-  if (tid == 0) scale[row] = s;
+  const RowScale sc = row_scale<TB>(top, red);
+  if (tid == 0) scale[row] = sc.s;
   for (int k0 = 0; k0 < K; k0 += TILE) {
 #pragma unroll
     for (int u = 0; u < kQP; ++u) {
       const int k = k0 + (u * TB + tid) * N;
       if (K > TILE) p[u].load(x, k, K, 0);
       uint32_t w[N / 4];
-#pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
-        w[i] = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[i] |= (uint32_t)((ok ? quant1(p[u].get(4 * i + e), s, inv) : 0) & 0xff) << (8 * e);
-      }
+      quant_piece<T>(p[u], sc, w);
       if (k + N <= K) {
         __builtin_memcpy(q + k, w, N);
       } else {
@@ -348,15 +365,46 @@ void launch_gemm(GemmArgs a, bool dw, bool dq, hipStream_t st) {
 // to 16 FN tokens; each wave streams an eighth of k from global memory straight into the matrix
 // instruction's operands (a lane has 16 bytes of one channel, 64 bytes of it lie in one instruction)
 // and the sums, whole numbers, are added in LDS.  The tokens' rows are small and come from the caches.
-constexpr int kSkinnyWaves = 8;
+// QUANT: each block quantises the tokens for itself, to LDS: up to kQuantMax values cost it less than
+// a launch before this one (one token of 4096: 7 us with it, 12 without).
+constexpr int kSkinnyWaves = 8, kQuantMax = 16384;
 
-template <class T, int FM, int FN>
-__global__ __launch_bounds__(64 * kSkinnyWaves) void int8_skinny_k(GemmArgs a) {
+template <class T, int FM, int FN, bool QUANT>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void int8_skinny_k(GemmArgs a, const typename T::store_t* x,
+                                                                   int64_t ldx) {
   __shared__ i32x4 part[kSkinnyWaves][FM * FN][64];
+  __shared__ __attribute__((aligned(16))) int8_t qs[QUANT ? kQuantMax + 16 * 80 : 16];
+  __shared__ float xs_s[16];
+  __shared__ uint32_t top_s[kSkinnyWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fc = lane >> 4;
+  const int pitch = (a.K + 63) / 64 * 64 + 16;  // of a token's row in LDS
+  if constexpr (QUANT) {
+    constexpr int N = Piece<T>::kN, TB = 64 * kSkinnyWaves;
+    for (int m = 0; m < (int)a.M; ++m) {
+      const typename T::store_t* xr = x + m * ldx;
+      uint32_t top = 0;
+      for (int k = tid * N; k < a.K; k += TB * N) {
+        Piece<T> p;
+        p.load(xr, k, a.K, 0);
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(p.get(e)) & 0x7fffffffu);
+      }
+      const RowScale sc = row_scale<TB>(top, top_s);
+      if (tid == 0) xs_s[m] = sc.s;
+      for (int k = tid * N; k < pitch - 16; k += TB * N) {
+        Piece<T> p;
+        p.load(xr, k, a.K, 0);  // zeros behind the end
+        uint32_t w[N / 4];
+        quant_piece<T>(p, sc, w);
+        __builtin_memcpy(qs + m * pitch + k, w, N);
+      }
+      __syncthreads();
+    }
+  }
   const int n0 = (blockIdx.x % a.tiles_n) * 16 * FM;
   const int64_t m0 = (int64_t)(blockIdx.x / a.tiles_n) * 16 * FN;
   const int8_t *pw[FM], *pq[FN];
+  const int8_t* ql = qs + min(fr, QUANT ? (int)a.M - 1 : 0) * pitch + 16 * fc;
 #pragma unroll
   for (int i = 0; i < FM; ++i) pw[i] = a.w + (int64_t)min(n0 + 16 * i + fr, a.N - 1) * a.ldw + 16 * fc;
 #pragma unroll
@@ -373,7 +421,8 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void int8_skinny_k(GemmArgs a) {
 #pragma unroll
       for (int i = 0; i < FM; ++i) fw[s][i] = load16(pw[i] + 64 * (u + s));
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fq[s][j] = load16(pq[j] + 64 * (u + s));
+      for (int j = 0; j < FN; ++j)
+        fq[s][j] = QUANT ? *reinterpret_cast<const i32x4*>(ql + 64 * (u + s)) : load16(pq[j] + 64 * (u + s));
     }
 #pragma unroll
     for (int s = 0; s < U; ++s)
@@ -388,7 +437,9 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void int8_skinny_k(GemmArgs a) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) fw[i] = row16(pw[i] - 16 * fc, true, 64 * u + 16 * fc, a.K);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) fq[j] = row16(pq[j] - 16 * fc, true, 64 * u + 16 * fc, a.K);
+    for (int j = 0; j < FN; ++j)
+      fq[j] = QUANT ? *reinterpret_cast<const i32x4*>(ql + 64 * u)
+                    : row16(pq[j] - 16 * fc, true, 64 * u + 16 * fc, a.K);
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -407,16 +458,17 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void int8_skinny_k(GemmArgs a) {
     for (int w = 1; w < kSkinnyWaves; ++w) v += part[w][g][l];
     const int64_t m = m0 + 16 * j + (l & 15);
     const int n = n0 + 16 * i + 4 * (l >> 4);
-    if (m < a.M && n < a.N) Four(a, n).put<T>(a, m, n, v, a.xs[m]);
+    if (m < a.M && n < a.N) Four(a, n).put<T>(a, m, n, v, QUANT ? xs_s[m] : a.xs[m]);
   }
 }
 
-template <class T, int FM, int FN>
-void launch_skinny(GemmArgs a, hipStream_t st) {
+template <class T, int FM, int FN, bool QUANT = false>
+void launch_skinny(GemmArgs a, hipStream_t st, const void* x = nullptr, int64_t ldx = 0) {
   a.tiles_n = cdiv(a.N, 16 * FM);
   const int64_t blocks = (a.M + 16 * FN - 1) / (16 * FN) * a.tiles_n;
   MX_CHECK(blocks <= kMaxRows, "linear_int8: too many tiles");
-  MX_LAUNCH((int8_skinny_k<T, FM, FN>), dim3((uint32_t)blocks), dim3(64 * kSkinnyWaves), 0, st, a);
+  MX_LAUNCH((int8_skinny_k<T, FM, FN, QUANT>), dim3((uint32_t)blocks), dim3(64 * kSkinnyWaves), 0, st, a,
+            static_cast<const typename T::store_t*>(x), ldx);
 }
 
 }  // namespace
@@ -467,6 +519,34 @@ void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, cons
     else if (c128x2 <= c256) launch_gemm<T, 128, 128, 2, 4, 2>(a, dw, dq, st);
     else launch_gemm<T, 256, 256, 2, 4, 2>(a, dw, dq, st);
   });
+}
+
+namespace {
+// tokens that the product's own kernel quantises
+bool quantises(int xtype, int ytype, int64_t M, int K) { return xtype == ytype && M <= 16 && M * K <= kQuantMax; }
+int64_t padded(int K) { return (K + 15) / 16 * 16; }
+}  // namespace
+
+int64_t linear_int8_scratch(int xtype, int ytype, int64_t M, int K) {
+  return quantises(xtype, ytype, M, K) ? 0 : M * (padded(K) + 4);
+}
+
+void linear_int8_float(const void* x, int xtype, int64_t ldx, const int8_t* w, int64_t ldw, int w_room, const float* ws,
+                       const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu, void* scratch,
+                       hipStream_t st) {
+  MX_CHECK(M >= 0 && M <= kMaxRows && N >= 1 && K >= 1 && K <= kInt8MaxK && ldw >= 0 && ldw <= kInt8MaxLd,
+           "linear_int8: bad sizes");
+  if (M == 0) return;
+  if (quantises(xtype, ytype, M, K)) {
+    GemmArgs a{nullptr, w, nullptr, ws, bias, y, 0, ldw, M, N, K, relu ? 1 : 0, 0, 0};
+    MX_BY_TYPE(ytype, T, (launch_skinny<T, 1, 1, true>(a, st, x, ldx)));
+    return;
+  }
+  MX_CHECK(scratch, "linear_int8: scratch needed");
+  int8_t* q = static_cast<int8_t*>(scratch);
+  float* s = reinterpret_cast<float*>(q + M * padded(K));
+  quantize_rows(x, xtype, ldx, q, padded(K), s, M, K, st);
+  linear_int8(q, padded(K), (int)padded(K), s, w, ldw, w_room, ws, bias, y, ytype, M, N, K, relu, st);
 }
 
 }  // namespace mx

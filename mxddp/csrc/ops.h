@@ -308,6 +308,12 @@ void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, cons
                  const float* ws, const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu,
                  hipStream_t st);
 
+// the same of float tokens, quantised on the way; scratch: linear_int8_scratch(...) bytes (0: none)
+int64_t linear_int8_scratch(int xtype, int ytype, int64_t M, int K);
+void linear_int8_float(const void* x, int xtype, int64_t ldx, const int8_t* w, int64_t ldw, int w_room, const float* ws,
+                       const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu, void* scratch,
+                       hipStream_t st);
+
 // ---- learning from a teacher (distill.hip) ----
 constexpr int kTopMax = 256;  // most top logits of a row
 // the k largest logits of each row in falling order (equal ones by index), their indices, and

@@ -14,8 +14,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import native
-from . import _native, _p, stream_of
-from .lowp import DTYPES, MAX_ROWS, check_device, check_float, on_device, rows_of
+from . import _native, _p
+from .lowp import DTYPES, MAX_ROWS, check_device, check_float, on_device, rows_of, stream
 
 MAX_TOP = 256       # csrc/ops.h kTopMax
 MAX_CLASSES = 2**30
@@ -65,7 +65,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
         n = C.top_logits_scratch(rows, V, k)
         scratch = torch.empty((n,), device=z.device, dtype=torch.int64) if n else None
         C.top_logits(z.data_ptr(), DTYPES[z.dtype], z.stride(0), rows, V, k, temperature, values.data_ptr(),
-                     index.data_ptr(), lse.data_ptr(), _p(scratch), stream_of(z))
+                     index.data_ptr(), lse.data_ptr(), _p(scratch), stream(z))
     return TopLogits(values, index, lse)
 
 
@@ -87,7 +87,7 @@ class _DistillLoss(torch.autograd.Function):
             n = C.distill_scratch(rows, z.shape[1])
             scratch = torch.empty((n,), device=z.device, dtype=torch.float32) if n else None
             C.distill_fwd(*_args(z, tv, ti, target, tlse, stats, temperature, hard), loss_rows.data_ptr(), _p(loss),
-                          reduction == "mean", _p(scratch), stream_of(z))
+                          reduction == "mean", _p(scratch), stream(z))
         ctx.save_for_backward(z, tv, ti, target, tlse, stats)
         ctx.args = (temperature, hard)
         ctx.per_row = loss is None
@@ -101,7 +101,7 @@ class _DistillLoss(torch.autograd.Function):
         dloss = dloss.to(torch.float32).contiguous()
         with on_device(z):
             native().distill_bwd(*_args(z, tv, ti, target, tlse, stats, *ctx.args), dloss.data_ptr(), ctx.per_row,
-                                 dz.data_ptr(), stream_of(z))
+                                 dz.data_ptr(), stream(z))
         return dz, None, None, None, None, None, None, None
 
 

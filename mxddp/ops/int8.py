@@ -9,9 +9,8 @@ from __future__ import annotations
 import torch
 
 from .. import native
-from .. import ops as _ops
-from . import _native, _p, stream_of
-from .lowp import DTYPES, MAX_ROWS, check_device, check_float, on_device, rows_of
+from . import _native, _p
+from .lowp import DTYPES, MAX_ROWS, check_device, check_float, on_device, rows_of, stream
 
 MAX_K = 2**17 - 1  # products of 2^14 each whose sum stays below 2^31
 _TINY = 2.0**-126
@@ -38,16 +37,13 @@ def quantize_rows(x: torch.Tensor):
     K = x.shape[-1]
     q = torch.empty(x.shape, device=x.device, dtype=torch.int8)
     scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    _quantize(rows_of(x), q, K, scale)
-    return q, scale
-
-
-def _quantize(x2, q, ldq, scale):
+    x2 = rows_of(x)
     if x2.shape[0] > MAX_ROWS:
         raise ValueError(f"quantize_rows: {x2.shape[0]} rows, at most {MAX_ROWS}")
     with on_device(x2):
-        native().quantize_rows(x2.data_ptr(), DTYPES[x2.dtype], x2.stride(0), q.data_ptr(), ldq, scale.data_ptr(),
-                               x2.shape[0], x2.shape[1], stream_of(x2))
+        native().quantize_rows(x2.data_ptr(), DTYPES[x2.dtype], x2.stride(0), q.data_ptr(), K, scale.data_ptr(),
+                               x2.shape[0], K, stream(x2))
+    return q, scale
 
 
 def _room(w, K):
@@ -109,16 +105,15 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     weight_scale = weight_scale.contiguous()
     bias = None if bias is None else bias.contiguous()
     y = torch.empty((*x.shape[:-1], N), device=x.device, dtype=out_dtype)
-    if given:
-        x2 = x2 if x2.stride(0) <= _MAX_LD else x2.contiguous()
-        q, ldq, s = x2, x2.stride(0), x_scale.contiguous()
-    else:
-        ldq = (K + 15) // 16 * 16
-        q = torch.empty((M, ldq), device=x.device, dtype=torch.int8)
-        s = torch.empty((M,), device=x.device, dtype=torch.float32)
-        _quantize(x2, q, ldq, s)
+    C, xt, yt = native(), DTYPES.get(x2.dtype, -1), DTYPES[out_dtype]
+    wargs = (weight.data_ptr(), weight.stride(0), _room(weight, K), weight_scale.data_ptr(), _p(bias), y.data_ptr(), yt,
+             M, N, K, bool(relu))
     with on_device(x2):
-        native().linear_int8(q.data_ptr(), ldq, K if given else ldq, s.data_ptr(), weight.data_ptr(), weight.stride(0),
-                             _room(weight, K), weight_scale.data_ptr(), _p(bias), y.data_ptr(), DTYPES[out_dtype], M,
-                             N, K, bool(relu), stream_of(x2))
+        if given:
+            x2 = x2 if x2.stride(0) <= _MAX_LD else x2.contiguous()
+            C.linear_int8(x2.data_ptr(), x2.stride(0), K, x_scale.contiguous().data_ptr(), *wargs, stream(x2))
+        else:
+            n = C.linear_int8_scratch(xt, yt, M, K)
+            scratch = torch.empty((n,), device=x2.device, dtype=torch.int8) if n else None
+            C.linear_int8_float(x2.data_ptr(), xt, x2.stride(0), *wargs, _p(scratch), stream(x2))
     return y

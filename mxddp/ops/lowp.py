@@ -27,8 +27,16 @@ def rows_of(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or n == 1 else t.contiguous()
 
 
+def stream(t: torch.Tensor) -> int:
+    """The current stream's handle, without the Stream object that ``ops.stream_of`` makes (1.8 us)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+_HERE = contextlib.nullcontext()
+
+
 def on_device(t: torch.Tensor):
     """Launches go to the current device: make it the tensor's."""
     if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(t.device)
