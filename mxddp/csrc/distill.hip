@@ -59,6 +59,45 @@ struct MaxSum {
 };
 
 constexpr int kT = 256;
+constexpr int kU = 4;  // pieces of 16 bytes a thread holds: a tile is TB * kU pieces
+
+// a thread's pieces of the tile at `base` (rows end at `end`); inside the row no lane looks at the end
+template <class T, int TB>
+__device__ __forceinline__ void load_tile(Piece<T>* x, const typename T::store_t* z, int base, int end) {
+  constexpr int N = Piece<T>::kN;
+  if (base + TB * kU * N <= end) {
+    const typename T::store_t* p = z + base + threadIdx.x * N;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const Bytes16 b = *reinterpret_cast<const Bytes16*>(p + u * TB * N);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[u].v[j] = b.v[j];
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) x[u].load(z, base + (u * TB + threadIdx.x) * N, end, T::kNegInf);
+  }
+}
+
+// The running sum of a thread's tiles: exponentials are exp2(z c - R), one fma each, with R the rounded
+// m c; `settle` takes the sum to m itself.  A row whose maximum times c leaves fp32 (only masked by a
+// type's lowest value, or as large) ends with s = 0 or an infinite R: it is summed again by MaxSum.
+struct TileSum {
+  float m = kLowest, s = 0.f, R = kLowest;
+  __device__ __forceinline__ void raise(float top, float c) {
+    if (top > m) {
+      m = top;
+      const float n = fmaxf(top * c, kLowest);
+      s *= exp2_raw(R - n);
+      R = n;
+    }
+  }
+  __device__ __forceinline__ float term(float z, float c) const { return exp2_raw(__builtin_fmaf(z, c, -R)); }
+  __device__ __forceinline__ float settled(float c) const {
+    return s > 0.f ? s * exp2_raw(-__builtin_fmaf(m, c, -R)) : s;
+  }
+};
+__device__ __forceinline__ bool unsettled(float m, float s, float c) { return !(s > 0.f) || !(fabsf(m * c) < INFINITY); }
 
 // over a block of TB threads; every thread gets the result
 template <int TB>
@@ -93,7 +132,6 @@ __device__ __forceinline__ MaxSum block_merge(MaxSum v, float c, float* red) {
 //
 // Few long rows are split over blocks: each leaves its segment's k largest keys, in order, and its
 // sum, and top_merge_k joins them.
-constexpr int kU = 4;  // pieces a thread holds
 // candidates: twice the largest k and more; a block of one wave has short rows, and many to a CU
 constexpr int top_cap(int tb) { return tb == 64 ? 512 : 1024; }
 // noted pieces: up to 2 k or 128 stay noted before a tile that may add all of its own
@@ -233,28 +271,27 @@ __global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
   const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
   const int gather = max(2 * k, 128);
   Candidates<TB> cand{buf[0], buf[1], slots, &cnt, 0, 0.f};
-  MaxSum ms;
+  TileSum ts;
   if (tid == 0) cnt = noted = 0;
 #pragma unroll 1
   for (int base = begin; base < end; base += TILE) {
     Piece<T> x[kU];
-    float top[kU];
-    bool odd[kU];  // the piece's sum is NaN: it may hold one, or infinities
-#pragma unroll
-    for (int u = 0; u < kU; ++u) x[u].load(z, base + (u * TB + tid) * N, end, T::kNegInf);
+    float top[kU], f[kU * N];
+    load_tile<T, TB>(x, z, base, end);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      float m = x[u].get(0);
 #pragma unroll
-      for (int e = 1; e < N; ++e) m = fmaxf(m, x[u].get(e));
-      top[u] = m;
-      ms.raise(m, a.c);
-      float s = 0.f;
+      for (int e = 0; e < N; ++e) f[u * N + e] = x[u].get(e);
+      top[u] = f[u * N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) s += exp2_raw((x[u].get(e) - ms.m) * a.c);
-      odd[u] = s != s;
-      ms.s += s;
+      for (int e = 1; e < N; ++e) top[u] = fmaxf(top[u], f[u * N + e]);
     }
+    ts.raise(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), a.c);
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < kU * N; ++e) s += ts.term(f[e], a.c);
+    ts.s += s;
+    const bool odd = s != s;  // the sum is NaN: there may be one, or infinities
     // the largest prefix that k of the tile's maxima reach (a piece of NaN alone counts as one)
     auto tile_prefix = [&] {
       uint32_t prefix = 0;
@@ -279,7 +316,7 @@ __global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int i0 = base + (u * TB + tid) * N;
-      if (i0 < end && (odd[u] || (first ? order_bits(top[u]) >= cand.floor : top[u] > cand.t)))
+      if (i0 < end && (odd || (first ? order_bits(top[u]) >= cand.floor : top[u] > cand.t)))
         piece[atomicAdd(&noted, 1)] = i0;
     }
     __syncthreads();
@@ -321,7 +358,15 @@ __global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
       __syncthreads();
     }
   }
+  MaxSum ms;
+  ms.m = ts.m;
+  ms.s = ts.settled(a.c);
   ms = block_merge<TB>(ms, a.c, red);
+  if (unsettled(ms.m, ms.s, a.c)) {
+    ms = MaxSum();
+    for (int i = begin + tid; i < end; i += TB) ms.add(T::load(z[i]), a.c);
+    ms = block_merge<TB>(ms, a.c, red);
+  }
   const int n = cand.n, kk = min(k, n);
   for (int i = tid; i < n; i += TB) {
     const uint64_t key = cand.list[i];
@@ -472,62 +517,82 @@ __device__ __forceinline__ Sums block_merge(Sums v, float c, float c1, float* re
   return t;
 }
 
-// classes [begin, end) of a row; `two`: both sums
+// classes [begin, end) of a row; `two`: both sums.  The mask has a word for each thread and tile, with
+// a bit for each of its elements.
 template <class T>
 __device__ __forceinline__ Sums row_sums(const DistillArgs& a, const typename T::store_t* z, int begin, int end,
                                          int cls, bool two, uint32_t* mask, float* red) {
-  constexpr int N = Piece<T>::kN;
+  constexpr int N = Piece<T>::kN, TILE = kT * kU * N;
   const int tid = threadIdx.x;
   const float c = (float)(kLog2e / a.temperature), c1 = (float)kLog2e;
   const bool tail = a.tlse != nullptr;
-  Sums v;
+  TileSum t, t1;
+  auto word = [](int i) { return i / TILE * kT + i / N % kT; };
+  auto bit = [](int i) { return i / (kT * N) % kU * N + i % N; };
+  auto set_mask = [&](int v0, int n) {
+    __syncthreads();
+    for (int i = tid; i < (n + TILE - 1) / TILE * kT; i += kT) mask[i] = 0;
+    __syncthreads();
+    if (cls >= v0 && cls < v0 + n) atomicOr(&mask[word(cls - v0)], 1u << bit(cls - v0));
+    __syncthreads();
+  };
   for (int v0 = begin; v0 < end; v0 += kMaskBits) {
     const int n = min(end - v0, kMaskBits);
-    if (tail) {
-      __syncthreads();
-      for (int i = tid; i < (n + 31) / 32; i += kT) mask[i] = 0;
-      __syncthreads();
-      if (cls >= v0 && cls < v0 + n) atomicOr(&mask[(cls - v0) >> 5], 1u << ((cls - v0) & 31));
-      __syncthreads();
-    }
-    for (int base = tid * N; base < n; base += kT * kU * N) {
+    if (tail) set_mask(v0, n);
+#pragma unroll 1
+    for (int base = 0; base < n; base += TILE) {
       Piece<T> x[kU];
+      float f[kU * N];
+      load_tile<T, kT>(x, z + v0, base, n);
 #pragma unroll
-      for (int u = 0; u < kU; ++u) x[u].load(z + v0, base + u * kT * N, n, T::kNegInf);
+      for (int u = 0; u < kU; ++u)
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const int i = base + u * kT * N;
-        float f[N];
+        for (int e = 0; e < N; ++e) f[u * N + e] = x[u].get(e);
+      if (tail) {
+        const uint32_t bits = mask[base / TILE * kT + tid];
+        if (bits) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = x[u].get(e);
-        if (tail && i < n) {
-          const uint32_t bits = mask[i >> 5] >> (i & 31);
-          if (bits & ((1u << N) - 1)) {
-#pragma unroll
-            for (int e = 0; e < N; ++e) f[e] = bits >> e & 1 ? -INFINITY : f[e];
-          }
+          for (int e = 0; e < kU * N; ++e) f[e] = bits >> e & 1 ? -INFINITY : f[e];
         }
-        float top = f[0];
+      }
+      float top = f[0], s = 0.f, s1 = 0.f;
 #pragma unroll
-        for (int e = 1; e < N; ++e) top = fmaxf(top, f[e]);
-        if (top > v.m) {
-          v.s *= exp2_raw((v.m - top) * c);
-          if (two) v.s1 *= exp2_raw((v.m - top) * c1);
-          v.m = top;
-        }
-        float s = 0.f, s1 = 0.f;
+      for (int e = 1; e < kU * N; ++e) top = fmaxf(top, f[e]);
+      t.raise(top, c);
 #pragma unroll
-        for (int e = 0; e < N; ++e) s += exp2_raw((f[e] - v.m) * c);
-        v.s += s;
-        if (two) {
+      for (int e = 0; e < kU * N; ++e) s += t.term(f[e], c);
+      t.s += s;
+      if (two) {
+        t1.raise(top, c1);
 #pragma unroll
-          for (int e = 0; e < N; ++e) s1 += exp2_raw((f[e] - v.m) * c1);
-          v.s1 += s1;
-        }
+        for (int e = 0; e < kU * N; ++e) s1 += t1.term(f[e], c1);
+        t1.s += s1;
       }
     }
   }
-  return block_merge(v, c, c1, red);
+  Sums v;
+  v.m = t.m;
+  v.s = t.settled(c);
+  v.s1 = two ? t1.settled(c1) : 0.f;
+  v = block_merge(v, c, c1, red);
+  if (unsettled(v.m, v.s, c) || (two && unsettled(v.m, v.s1, c1))) {
+    MaxSum o, o1;
+    for (int v0 = begin; v0 < end; v0 += kMaskBits) {
+      const int n = min(end - v0, kMaskBits);
+      if (tail) set_mask(v0, n);
+      for (int i = tid; i < n; i += kT) {
+        if (tail && (mask[word(i)] >> bit(i) & 1)) continue;
+        const float x = T::load(z[v0 + i]);
+        o.add(x, c);
+        if (two) o1.add(x, c1);
+      }
+    }
+    v.m = o.m;
+    v.s = o.s;
+    v.s1 = two ? o1.s : 0.f;
+    v = block_merge(v, c, c1, red);
+  }
+  return v;
 }
 
 struct RowShared {
