@@ -148,6 +148,32 @@ struct TopArgs {
   float c, inv_t;
 };
 
+// The largest 16-bit prefix p that at least k of a block's values reach, 0 if there are fewer values.
+// Two bits a round: count(trial) is a wave's number of values whose prefix is >= trial; the three
+// counts of a round (each below 2^20) share a word.  `slots` holds two rounds, so one barrier a round
+// is enough.
+template <int TB, class F>
+__device__ __forceinline__ uint32_t prefix_of(int k, uint64_t* slots, F count) {
+  uint32_t p = 0;
+#pragma unroll 1
+  for (int bit = 14; bit >= 0; bit -= 2) {
+    uint64_t c = 0;
+#pragma unroll
+    for (uint32_t i = 1; i < 4; ++i) c |= (uint64_t)count(p | i << bit) << (20 * (i - 1));
+    if constexpr (TB > 64) {
+      uint64_t* s = slots + (bit >> 1 & 1) * (TB / 64);
+      if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = c;
+      __syncthreads();
+      c = 0;
+#pragma unroll
+      for (int w = 0; w < TB / 64; ++w) c += s[w];
+    }
+    const uint32_t m = (1u << 20) - 1;
+    const uint32_t i = (int)(c >> 40 & m) >= k ? 3 : (int)(c >> 20 & m) >= k ? 2 : (int)(c & m) >= k ? 1 : 0;
+    p |= i << bit;
+  }
+  return p;
+}
 __device__ __forceinline__ int wave_count(bool b) { return __popcll(__ballot(b)); }
 // a block's total of its waves' counts.  `slots` holds two rounds, so one barrier a round is enough.
 template <int TB>
@@ -210,7 +236,7 @@ template <int TB>
 struct Candidates {
   uint64_t* list;
   uint64_t* other;
-  int* slots;
+  uint64_t* wide;
   int* cnt;
   int n;
   float t;             // a further element has to be above it
@@ -219,14 +245,11 @@ struct Candidates {
   // keep those that reach the largest 16-bit prefix that k of them reach
   __device__ __forceinline__ void raise(int k) {
     const int tid = threadIdx.x;
-    uint32_t prefix = 0;
-#pragma unroll 1
-    for (int bit = 15; bit >= 0; --bit) {
-      const uint32_t trial = prefix | 1u << bit;
+    const uint32_t prefix = prefix_of<TB>(k, wide, [&](uint32_t trial) {
       int c = 0;
       for (int i = tid; i < (n + 63) / 64 * 64; i += TB) c += wave_count(i < n && (uint32_t)(list[i] >> 48) >= trial);
-      if (block_count<TB>(c, slots, bit) >= k) prefix = trial;
-    }
+      return c;
+    });
     if (tid == 0) *cnt = 0;
     __syncthreads();
     for (int i = tid; i < n; i += TB)
@@ -243,6 +266,24 @@ struct Candidates {
     other = l;
   }
 };
+
+// Each candidate's place, the number of larger keys, to put(place, key).  Eight keys a step, so a step
+// waits once for LDS; the list is filled up with zeros, which are below every key.
+template <int TB, class F>
+__device__ __forceinline__ void rank_all(uint64_t* list, int n, F put) {
+  const int tid = threadIdx.x, n8 = (n + 7) / 8 * 8;
+  if (n + tid < n8) list[n + tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += TB) {
+    const uint64_t key = list[i];
+    int place = 0;
+    for (int j = 0; j < n8; j += 8) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) place += list[j + e] > key;
+    }
+    put(place, key);
+  }
+}
 
 // the row's rank-th answer; the first one's writer has the sum: an infinite or NaN maximum is its value
 template <class T>
@@ -261,16 +302,17 @@ template <class T, int TB>
 __global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
   constexpr int N = Piece<T>::kN, TILE = TB * kU * N, kCap = top_cap(TB);
   static_assert(kCap >= 2 * kTopMax, "a list that was cut to k leaves half of its room");
-  __shared__ uint64_t buf[2][kCap];
+  __shared__ __attribute__((aligned(16))) uint64_t buf[2][kCap];
   __shared__ int piece[top_pieces(TB)];
   __shared__ int slots[2 * TB / 64], cnt, noted;
+  __shared__ uint64_t wide[2 * TB / 64];
   __shared__ float red[2 * TB / 64];
   const int tid = threadIdx.x, k = a.k;
   const int64_t row = blockIdx.x / a.nseg;
   const int seg = blockIdx.x % a.nseg, begin = seg * a.seglen, end = min(a.V, begin + a.seglen);
   const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
   const int gather = max(2 * k, 128);
-  Candidates<TB> cand{buf[0], buf[1], slots, &cnt, 0, 0.f};
+  Candidates<TB> cand{buf[0], buf[1], wide, &cnt, 0, 0.f};
   TileSum ts;
   if (tid == 0) cnt = noted = 0;
 #pragma unroll 1
@@ -294,17 +336,16 @@ __global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
     const bool odd = s != s;  // the sum is NaN: there may be one, or infinities
     // the largest prefix that k of the tile's maxima reach (a piece of NaN alone counts as one)
     auto tile_prefix = [&] {
-      uint32_t prefix = 0;
-#pragma unroll 1
-      for (int bit = 15; bit >= 0; --bit) {
-        const uint32_t trial = prefix | 1u << bit;
-        int c = 0;
+      uint32_t key[kU];
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
-          c += wave_count(base + (u * TB + tid) * N < end && order_bits(top[u]) >> 16 >= trial);
-        if (block_count<TB>(c, slots, bit) >= k) prefix = trial;
-      }
-      return prefix << 16;
+      for (int u = 0; u < kU; ++u)
+        key[u] = base + (u * TB + tid) * N < end ? order_bits(top[u]) >> 16 : 0;
+      return prefix_of<TB>(k, wide, [&](uint32_t trial) {
+               int c = 0;
+#pragma unroll
+               for (int u = 0; u < kU; ++u) c += wave_count(key[u] >= trial);
+               return c;
+             }) << 16;
     };
     const bool first = base == begin;
     const int before = noted;
@@ -344,7 +385,8 @@ __global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
       cand.n = cnt;
       __syncthreads();  // every thread has read both counters
       cand.t = from_order_bits(cand.floor);
-      if (cand.n <= kCap && cand.n > k + 16) cand.raise(k);
+      // the last candidates are ordered: worth it only where there are many
+      if (cand.n <= kCap && cand.n > (last ? k + 192 : k + 16)) cand.raise(k);
       if (cand.n > (last ? kCap : kCap / 2)) {
         const bool over = cand.n > kCap;  // the list is what it was before, the rest is in the pieces
         const uint64_t low = select_exact<T, TB>(cand.list, over ? had : cand.n, cand.other, z, piece, over ? np : 0,
@@ -367,15 +409,12 @@ __global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
     for (int i = begin + tid; i < end; i += TB) ms.add(T::load(z[i]), a.c);
     ms = block_merge<TB>(ms, a.c, red);
   }
-  const int n = cand.n, kk = min(k, n);
-  for (int i = tid; i < n; i += TB) {
-    const uint64_t key = cand.list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += cand.list[j] > key;
-    if (rank >= kk) continue;
+  const int kk = min(k, cand.n);
+  rank_all<TB>(cand.list, cand.n, [&](int rank, uint64_t key) {
+    if (rank >= kk) return;
     if (a.nseg == 1) put_top<T>(a, row, rank, key, z, ms);
     else a.part[(row * a.nseg + seg) * k + rank] = key;
-  }
+  });
   if (a.nseg > 1) {
     for (int i = kk + tid; i < k; i += TB) a.part[(row * a.nseg + seg) * k + i] = 0;
     if (tid == 0) reinterpret_cast<float2*>(a.part + a.rows * a.nseg * k)[row * a.nseg + seg] = make_float2(ms.m, ms.s);
@@ -387,22 +426,26 @@ __global__ __launch_bounds__(TB) void top_logits_k(TopArgs a) {
 template <class T>
 __global__ __launch_bounds__(kT) void top_merge_k(TopArgs a) {
   constexpr int kCap = top_cap(kT);
-  __shared__ uint64_t buf[2][kCap];
+  __shared__ __attribute__((aligned(16))) uint64_t buf[2][kCap];
   __shared__ int slots[2 * kT / 64], cnt;
+  __shared__ uint64_t wide[2 * kT / 64];
   __shared__ float red[2 * kT / 64];
   const int tid = threadIdx.x, k = a.k, total = a.nseg * k;
   const int64_t row = blockIdx.x;
   const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
   const uint64_t* keys = a.part + row * total;
-  Candidates<kT> cand{buf[0], buf[1], slots, &cnt, 0, 0.f};
+  Candidates<kT> cand{buf[0], buf[1], wide, &cnt, 0, 0.f};
   MaxSum ms;
-  const int each = (k + a.nseg - 1) / a.nseg;
-  uint64_t least = ~0ull, last = 0;
-  for (int s = 0; s < a.nseg; ++s) {
-    const uint64_t x = keys[s * k + each - 1], y = keys[s * k + k - 1];
+  const int each = (k + a.nseg - 1) / a.nseg, lane = tid & 63;  // nseg <= 32
+  uint64_t least = lane < a.nseg ? keys[lane * k + each - 1] : ~0ull, last = lane < a.nseg ? keys[lane * k + k - 1] : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint64_t x = __shfl_xor((unsigned long long)least, o, 32), y = __shfl_xor((unsigned long long)last, o, 32);
     least = x < least ? x : least;
     last = y > last ? y : last;
   }
+  least = __shfl((unsigned long long)least, 0, 64);
+  last = __shfl((unsigned long long)last, 0, 64);
   const uint64_t floor = least > last ? least : last;
   if (tid < a.nseg) {
     const float2 p = reinterpret_cast<const float2*>(a.part + a.rows * total)[row * a.nseg + tid];
@@ -422,15 +465,12 @@ __global__ __launch_bounds__(kT) void top_merge_k(TopArgs a) {
   if (cand.n > kCap) {
     select_exact<T, kT>(keys, total, cand.list, z, nullptr, 0, 0, k, slots, &cnt);
     cand.n = k;
-  } else if (cand.n > k + 64) {
+  } else if (cand.n > k + 192) {
     cand.raise(k);
   }
-  for (int i = tid; i < cand.n; i += kT) {
-    const uint64_t key = cand.list[i];
-    int rank = 0;
-    for (int j = 0; j < cand.n; ++j) rank += cand.list[j] > key;
+  rank_all<kT>(cand.list, cand.n, [&](int rank, uint64_t key) {
     if (rank < k) put_top<T>(a, row, rank, key, z, ms);
-  }
+  });
 }
 
 // blocks of a row: long rows that alone would not fill the machine are cut into pieces of 8,192
@@ -630,7 +670,10 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, co
   Sums all = out;
   if (tail) {  // and the named ones, each class once
     bool first = r.cls >= 0;
-    for (int j = 0; j < a.k && j < tid; ++j) first = first && sh.cls[j] != r.cls;
+    for (int j = 0; j < a.k; j += 8) {  // threads without an entry hold -1
+#pragma unroll
+      for (int e = 0; e < 8; ++e) first = first && (j + e >= tid || sh.cls[j + e] != r.cls);
+    }
     Sums in;
     if (first && !(zc < kLowest)) {
       in.m = zc == zc ? zc : kLowest;
@@ -830,7 +873,10 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
   __syncthreads();  // also orders the stores above before the ones below
   if (cls >= begin && cls < end) {
     float p = 0;  // a class that is named twice has both entries' share
-    for (int j = 0; j < a.k; ++j) p += cls_s[j] == cls ? p_s[j] : 0.f;
+    for (int j = 0; j < a.k; j += 8) {  // threads without an entry hold -1
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p += cls_s[j + e] == cls ? p_s[j + e] : 0.f;
+    }
     const float v = T::load(z[cls]);
     const float q = ci == 0.f ? 0.f : ci * exp2f((v - m) * c);
     float d = q - p;
@@ -839,7 +885,10 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
   }
   if (tid == 0 && y >= begin && y < end) {
     bool named = false;
-    for (int j = 0; j < a.k; ++j) named = named || cls_s[j] == y;
+    for (int j = 0; j < a.k; j += 8) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) named = named || cls_s[j + e] == y;
+    }
     if (!named) {
       const float v = T::load(z[y]);
       float d = co * fminf(exp2f((v - ref) * c), lim);
