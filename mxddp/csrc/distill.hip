@@ -61,6 +61,10 @@ struct MaxSum {
 constexpr int kT = 256;
 constexpr int kU = 4;  // pieces of 16 bytes a thread holds: a tile is TB * kU pieces
 
+// 16 bytes at any address, past the caches: a pass reads or writes a row once.  A distillation step of
+// 4096 x 131072 in bf16: 678 us with ordinary accesses, 667 with these loads, 600 with the stores too.
+typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(1)));
+
 // a thread's pieces of the tile at `base` (rows end at `end`); inside the row no lane looks at the end
 template <class T, int TB>
 __device__ __forceinline__ void load_tile(Piece<T>* x, const typename T::store_t* z, int base, int end) {
@@ -69,9 +73,9 @@ __device__ __forceinline__ void load_tile(Piece<T>* x, const typename T::store_t
     const typename T::store_t* p = z + base + threadIdx.x * N;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const Bytes16 b = *reinterpret_cast<const Bytes16*>(p + u * TB * N);
+      const any16 b = __builtin_nontemporal_load(reinterpret_cast<const any16*>(p + u * TB * N));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[u].v[j] = b.v[j];
+      for (int j = 0; j < 4; ++j) x[u].v[j] = b[j];
     }
   } else {
 #pragma unroll
@@ -737,7 +741,7 @@ __device__ __forceinline__ void leave_out(const DistillArgs& a, int64_t row, flo
 
 // part == nullptr: a block has the whole row; else [rows][nseg] sums of a segment each, for distill_join_k
 template <class T>
-__global__ __launch_bounds__(kT) void distill_fwd_k(DistillArgs a, int nseg, int seglen, float* __restrict__ part,
+__global__ __launch_bounds__(kT, 8) void distill_fwd_k(DistillArgs a, int nseg, int seglen, float* __restrict__ part,
                                                     float* __restrict__ loss_rows) {
   __shared__ RowShared sh;
   __shared__ uint32_t mask[kMaskBits / 32];
@@ -840,13 +844,14 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
   const float ref = st[0], co = st[1], m = st[2], ci = st[3], h1 = st[4];
   // without a share (co = 0) a named class above `ref` must not make a NaN of an overflow
   const float lim = co == 0.f ? 0.f : INFINITY;
-  for (int base = begin + tid * N; base < end; base += kT * kU * N) {
+  constexpr int TILE = kT * kU * N;
+#pragma unroll 1
+  for (int base = begin; base < end; base += TILE) {
     Piece<T> x[kU];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) x[u].load(z, base + u * kT * N, end, T::kNegInf);
+    load_tile<T, kT>(x, z, base, end);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int i = base + u * kT * N;
+      const int i = base + (u * kT + tid) * N;
       typename T::store_t o[N];
 #pragma unroll
       for (int e = 0; e < N; ++e) {
@@ -856,7 +861,9 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
         o[e] = T::store(g * d);
       }
       if (i + N <= end) {
-        __builtin_memcpy(dz + i, o, 16);
+        any16 w;
+        __builtin_memcpy(&w, o, 16);
+        __builtin_nontemporal_store(w, reinterpret_cast<any16*>(dz + i));
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)

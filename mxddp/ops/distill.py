@@ -78,29 +78,31 @@ def _args(z, tv, ti, target, tlse, stats, temperature, hard):
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, tv, ti, target, tlse, temperature, hard, reduction):
-        rows = z.shape[0]
-        stats = torch.empty((8 * rows + 1,), device=z.device, dtype=torch.float32)
-        loss_rows = torch.empty((rows,), device=z.device, dtype=torch.float32)
-        loss = torch.empty((), device=z.device, dtype=torch.float32) if reduction != "none" else None
+        C, (rows, V) = native(), z.shape
+        # the rows' statistics and weight for the backward, then what is used up here: the rows'
+        # losses (the result itself without a reduction) and the sums of a split row
+        n = 8 * rows + 1
+        buf = torch.empty((n + rows + C.distill_scratch(rows, V),), device=z.device, dtype=torch.float32)
+        loss = torch.empty(() if reduction != "none" else (rows,), device=z.device, dtype=torch.float32)
+        per_row = reduction == "none"
+        p = buf.data_ptr()
         with on_device(z):
-            C = native()
-            n = C.distill_scratch(rows, z.shape[1])
-            scratch = torch.empty((n,), device=z.device, dtype=torch.float32) if n else None
-            C.distill_fwd(*_args(z, tv, ti, target, tlse, stats, temperature, hard), loss_rows.data_ptr(), _p(loss),
-                          reduction == "mean", _p(scratch), stream(z))
-        ctx.save_for_backward(z, tv, ti, target, tlse, stats)
+            C.distill_fwd(*_args(z, tv, ti, target, tlse, buf, temperature, hard),
+                          loss.data_ptr() if per_row else p + 4 * n, 0 if per_row else loss.data_ptr(),
+                          reduction == "mean", p + 4 * (n + rows), stream(z))
+        ctx.save_for_backward(z, tv, ti, target, tlse, buf)
         ctx.args = (temperature, hard)
-        ctx.per_row = loss is None
-        return loss_rows if loss is None else loss
+        ctx.per_row = per_row
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        z, tv, ti, target, tlse, stats = ctx.saved_tensors
+        z, tv, ti, target, tlse, buf = ctx.saved_tensors
         dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
-        dloss = dloss.to(torch.float32).contiguous()
+        dloss = dloss.contiguous()
         with on_device(z):
-            native().distill_bwd(*_args(z, tv, ti, target, tlse, stats, *ctx.args), dloss.data_ptr(), ctx.per_row,
+            native().distill_bwd(*_args(z, tv, ti, target, tlse, buf, *ctx.args), dloss.data_ptr(), ctx.per_row,
                                  dz.data_ptr(), stream(z))
         return dz, None, None, None, None, None, None, None
 
