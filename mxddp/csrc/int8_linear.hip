@@ -6,6 +6,8 @@
 // the smaller one's last place), says which way.
 // int8_gemm_k: rows of q and rows of w, both contiguous in k, on v_mfma_i32_16x16x64_i8; the sum is a
 // whole number below 2^31, so it is exact in any order.
+#include <type_traits>
+
 #include "lowp.h"
 #include "ops.h"
 
@@ -204,7 +206,9 @@ __device__ __forceinline__ void wait_vm() {
 // token.
 // The fragments of one half stage are read while the other half's are multiplied.  The barrier stands
 // in the middle of a stage, where its second half is in registers: its buffer is free for stage
-// t + NS there, and the first half of stage t + 1 is read behind it.
+// t + NS there, and the first half of stage t + 1 is read behind it.  Reads and copies are issued one by
+// one between the matrix instructions: a copy of 1 KB keeps its wave from issuing for 16 cycles and
+// more, and all of a stage's in a row leave the matrix units idle for half a stage.
 template <class T, int TM, int TN, int WM, int WN, int NS, bool DW, bool DQ>
 __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
   constexpr int NW = WM * WN, FM = TM / WM / 16, FN = TN / WN / 16;
@@ -233,17 +237,20 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
 
   const auto rsw = tile_rsrc(wbase), rsq = tile_rsrc(qbase);
   i32x4 rw[DW ? 1 : IA], rq[DQ ? 1 : IB];
-  // straight to LDS
-  auto fetch = [&](int t, int buf) {
+  // straight to LDS: copy j of a stage's
+  constexpr int kCopies = (DW ? IA : 0) + (DQ ? IB : 0);
+  auto copy = [&](int t, int buf, int j) {
     const int k0 = t * 128;
-    // pieces behind the end of k are the stage's first: `read` clears the tokens' side of them
+    // pieces behind the end of k are the stage's first: `clear` takes the tokens' side of them out
     const uint32_t back = k0 + chunk < a.K ? 0 : chunk;
     char* st = sm + buf * SB;
+    const int i = DW ? j - IA : j;
+    if (DW && j < IA) glds16(rsw, offw[j] - back, k0, st + (wave * IA + j) * 1024);
+    else glds16(rsq, offq[i] - back, k0, st + TM * 128 + (wave * IB + i) * 1024);
+  };
+  auto fetch = [&](int t, int buf) {
 #pragma unroll
-    for (int j = 0; j < (DW ? IA : 0); ++j) glds16(rsw, offw[j] - back, k0, st + (wave * IA + j) * 1024);
-#pragma unroll
-    for (int j = 0; j < (DQ ? IB : 0); ++j)
-      glds16(rsq, offq[j] - back, k0, st + TM * 128 + (wave * IB + j) * 1024);
+    for (int j = 0; j < kCopies; ++j) copy(t, buf, j);
   };
   // to registers, and from there to LDS
   auto load = [&](int t) {
@@ -267,12 +274,13 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
   };
   const int fr = lane & 15, fc = lane >> 4;
   const int rw0 = (wm * FM * 16 + fr) * 128, rq0 = TM * 128 + (wn * FN * 16 + fr) * 128;
-  auto read = [&](int t, int buf, int half, i32x4* fw, i32x4* fq) {
+  // fragment r of a half stage: the tokens' first
+  auto read = [&](int buf, int half, int r, i32x4* fw, i32x4* fq) {
     const char* st = sm + buf * SB + 16 * ((4 * half + fc) ^ (fr & 7));
-#pragma unroll
-    for (int i = 0; i < FM; ++i) fw[i] = *reinterpret_cast<const i32x4*>(st + rw0 + i * 2048);
-#pragma unroll
-    for (int j = 0; j < FN; ++j) fq[j] = *reinterpret_cast<const i32x4*>(st + rq0 + j * 2048);
+    if (r < FN) fq[r] = *reinterpret_cast<const i32x4*>(st + rq0 + r * 2048);
+    else fw[r - FN] = *reinterpret_cast<const i32x4*>(st + rw0 + (r - FN) * 2048);
+  };
+  auto clear = [&](int t, int half, i32x4* fq) {
     if (DQ && t * 128 + 128 > a.K) {
       const bool ok = t * 128 + 64 * half + 16 * fc < a.K;
 #pragma unroll
@@ -280,12 +288,26 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
     }
   };
   i32x4 acc[FM][FN] = {};
-  auto mul = [&](const i32x4* fw, const i32x4* fq) {
+  // the products of (fw, fq); between them the reads of half a stage to (nw, nq) and the copies of stage t2
+  auto products = [&](auto more, auto copies, const i32x4* fw, const i32x4* fq, int nbuf, int nhalf, i32x4* nw,
+                      i32x4* nq, int t2, int cbuf) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int i = 0; i < FM; ++i) {
+      if constexpr (more.value) {
+#pragma unroll
+        for (int r = i * (FM + FN) / FM; r < (i + 1) * (FM + FN) / FM; ++r) read(nbuf, nhalf, r, nw, nq);
+      }
+      if constexpr (copies.value) {
+#pragma unroll
+        for (int j = i * kCopies / FM; j < (i + 1) * kCopies / FM; ++j) copy(t2, cbuf, j);
+      }
 #pragma unroll
       for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fq[j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
 
   const int nt = (a.K + 127) / 128;
   // through registers a stage is loaded behind the barrier before its turn and put in its place in the
@@ -309,28 +331,28 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
   }
   lds_barrier();
   i32x4 w0[FM], q0[FN], w1[FM], q1[FN];
-  read(0, 0, 0, w0, q0);
+#pragma unroll
+  for (int r = 0; r < FM + FN; ++r) read(0, 0, r, w0, q0);
   int buf = 0;
-  for (int t = 0; t < nt; ++t) {
+  // a stage with another behind it, with or without one to copy
+  auto stage = [&](auto copies, int t) {
     const int next = buf + 1 == NS ? 0 : buf + 1;
-    read(t, buf, 1, w1, q1);
-    mul(w0, q0);
-    if (t + 1 < nt) {
-      if constexpr (kDma) {  // stage t + 1 has landed; up to NS - 2 later ones are under way
-        if (t + NS <= nt) wait_vm<(NS - 2) * (IA + IB)>();
-        else wait_vm<0>();
-      } else {
-        put(t + 1, next);
-        wait_vm<0>();
-      }
-      lds_barrier();
-      if (t + kAhead < nt) fetch(t + kAhead, buf);
-      if constexpr (!kDma) load(min(t + 2, nt - 1));
-      read(t + 1, next, 0, w0, q0);
-    }
-    mul(w1, q1);
+    products(yes, no, w0, q0, buf, 1, w1, q1, 0, 0);
+    if constexpr (!kDma) put(t + 1, next);
+    // stage t + 1 has landed; up to NS - 2 later ones are under way
+    wait_vm<kDma && copies.value ? (NS - 2) * (IA + IB) : 0>();
+    lds_barrier();
+    if constexpr (!kDma) load(min(t + 2, nt - 1));
+    products(yes, copies, w1, q1, next, 0, w0, q0, t + kAhead, buf);
     buf = next;
-  }
+  };
+  int t = 0;
+  for (; t + kAhead < nt; ++t) stage(yes, t);
+  for (; t + 1 < nt; ++t) stage(no, t);
+  clear(t, 0, q0);
+  products(yes, no, w0, q0, buf, 1, w1, q1, 0, 0);
+  clear(t, 1, q1);
+  products(no, no, w1, q1, 0, 0, w0, q0, 0, 0);
   float xs[FN];
 #pragma unroll
   for (int j = 0; j < FN; ++j) xs[j] = a.xs[min<int64_t>(m0 + (wn * FN + j) * 16 + fr, a.M - 1)];
