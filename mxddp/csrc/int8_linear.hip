@@ -533,9 +533,17 @@ void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, cons
   const double c64 = 0.55 * rounds(64, 2 * cu), c128 = 0.8 * rounds(128, cu), c128x2 = 1.1 * rounds(128, 2 * cu);
   const double c256 = dw && dq ? 1.8 * rounds(256, cu) : 1e30;
   MX_BY_TYPE(ytype, T, {
-    // few tokens: the weight's bytes, at 4.5 TB/s; 32 tokens of 4096 x 4096 9 us, 19 on tiles
-    if (M <= 16 || K < 16) launch_skinny<T, 1, 1>(a, st);
-    else if (M <= 32) launch_skinny<T, 1, 2>(a, st);
+    // Few tokens: the weight's bytes, and for each block the tokens'.  Twice the channels a block halve
+    // the latter, where that leaves a block a CU: 16 tokens of 8192 x 8192 16 us (19 without), of 4096 x
+    // 4096 9 us (7 without); 32 tokens of 4096 x 4096 9 us, on tiles 19.
+    const bool wide = M > 8 && N >= 32 * cu;
+    if (M <= 16 || K < 16) {
+      if (wide) launch_skinny<T, 2, 1>(a, st);
+      else launch_skinny<T, 1, 1>(a, st);
+    } else if (M <= 32) {
+      if (wide) launch_skinny<T, 2, 2>(a, st);
+      else launch_skinny<T, 1, 2>(a, st);
+    }
     else if (c64 <= c128 && c64 <= c128x2 && c64 <= c256) launch_gemm<T, 64, 64, 2, 2, 4>(a, dw, dq, st);
     else if (c128 <= c128x2 && c128 <= c256 && dw && dq) launch_gemm<T, 128, 128, 2, 4, 4>(a, dw, dq, st);
     else if (c128x2 <= c256) launch_gemm<T, 128, 128, 2, 4, 2>(a, dw, dq, st);

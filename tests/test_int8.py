@@ -128,6 +128,32 @@ def test_linear_int8(dev, M, N, K):
     check_linear(ops.linear_int8(*args, b.to(dev), relu=True), q, s, w, ws, b, True)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N", [(2309, 4100), (1000, 4000), (1100, 4100), (520, 3970), (20, 8200), (9, 8197)])
+@pytest.mark.parametrize("K", [7, 16, 112, 128, 144, 250, 256, 384, 520, 640, 1008])
+def test_linear_int8_tiles(cuda, M, N, K):
+    """Every tile kernel (their choice goes by rounds over the machine), one stage of k to eight, k that
+    ends in a stage, in a piece, and rows of no alignment; the oracle's product in 64 bits is exact."""
+    g = torch.Generator(device=cuda).manual_seed(M + K)
+    q = torch.randint(-127, 128, (M, K), generator=g, dtype=torch.int8, device=cuda)
+    w = torch.randint(-127, 128, (N, K), generator=g, dtype=torch.int8, device=cuda)
+    s, ws = torch.rand(M, generator=g, device=cuda), torch.rand(N, generator=g, device=cuda) * 1e-3
+    b = torch.randn(N, generator=g, device=cuda)
+    prod = (q.double() @ w.double().t().contiguous()) * s.double()[:, None] * ws.double()
+    want = prod + b.double()
+    y = ops.linear_int8(q, w, ws, b, x_scale=s)
+    tol = 4.02 * E * prod.abs() + 1.01 * E * (b.double().abs() + want.abs())
+    assert bool(((y.double() - want).abs() <= tol).all())
+    # float tokens whose quantised values these are: rows of 127 at some place, a scale of 2^-7
+    x = q.float()
+    x[:, K // 2] = 127
+    prod = (x.double() @ w.double().t().contiguous()) * 2.0**-7 * ws.double()
+    y = ops.linear_int8((x * 2.0**-7).to(torch.bfloat16), w, ws, b, out_dtype=torch.float32)
+    want = prod + b.double()
+    tol = 4.02 * E * prod.abs() + 1.01 * E * (b.double().abs() + want.abs())
+    assert bool(((y.double() - want).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("M,N,K", [(1, 300, 1024), (5, 77, 96), (5, 77, 99), (70, 200, 1000), (300, 300, 512)])
 @pytest.mark.parametrize("out", TYPES)
