@@ -671,8 +671,12 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, co
   const bool tail = a.tlse != nullptr, two = a.hard > 0 && a.temperature != 1.0;
   float* st = a.stats + row * kDistillStats;
   const float zc = r.cls >= 0 ? T::load(z[r.cls]) : 0.f;
-  Sums all = out;
-  if (tail) {  // and the named ones, each class once
+  // all classes: those outside and the named ones, each class once.  Added in 64 bits, so the shares of
+  // the two sets are as near to each other as their sums say.
+  const bool has_out = out.s > 0.f || out.s != out.s;
+  float top = out.m;
+  double all_s = out.s, all_s1 = out.s1;
+  if (tail) {
     bool first = r.cls >= 0;
     for (int j = 0; j < a.k; j += 8) {  // threads without an entry hold -1
 #pragma unroll
@@ -684,9 +688,12 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, co
       in.s = in.s1 = zc == zc ? 1.f : zc;
     }
     in = block_merge(in, c, c1, sh.red);
-    all.merge(in.m, in.s, in.s1, c, c1);
+    top = fmaxf(out.m, in.m);
+    const double d = (double)out.m - top, e = (double)in.m - top;
+    all_s = out.s * exp(d * inv_t) + in.s * exp(e * inv_t);
+    if (two) all_s1 = out.s1 * exp(d) + in.s1 * exp(e);
   }
-  const double log_z = log((double)all.s);
+  const double log_z = log(all_s);
   // the teacher
   double norm = 0;
   if (tail) {
@@ -703,30 +710,29 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, co
   }
   const double p = r.cls >= 0 ? exp(r.u - norm) : 0.0;
   // p = 0 has no term, whatever the student's value
-  double kd = block_sum_d(p == 0 ? 0.0 : p * ((r.u - norm) - (((double)zc - all.m) * inv_t - log_z)), sh.redd);
+  double kd = block_sum_d(p == 0 ? 0.0 : p * ((r.u - norm) - (((double)zc - top) * inv_t - log_z)), sh.redd);
   const double named = tail ? block_sum_d(p, sh.redd) : 1.0;
   if (tid != 0) return;
-  // exp2((z - out.m) c) * co: the share of a class outside
-  const bool has_out = out.s > 0.f || out.s != out.s;
+  // exp2((z - ref) c) * co: what a class outside gets
   double mass = tail ? named : r.any ? 1.0 : 0.0, rest = 0.0;
-  const double shift = ((double)out.m - all.m) * inv_t;
+  const double shift = ((double)out.m - top) * inv_t;
   if (tail && has_out && !(named >= 1)) {
     rest = 1.0 - named;
     kd += rest * (log(rest) - (shift + log((double)out.s) - log_z));
     mass = 1.0;
   }
-  const double co = has_out ? mass * exp(shift) / all.s - (tail ? rest / out.s : 0.0)
-                    : all.s > 0.f ? 0.0 : __builtin_nan("");  // a row of -inf has no distribution
-  const float ref = has_out ? out.m : all.m;
-  const double h = a.hard, z1 = two ? (double)all.s1 : (double)all.s;
+  const double co = has_out ? mass * exp(shift) / all_s - (tail ? rest / out.s : 0.0)
+                    : all_s > 0 ? 0.0 : __builtin_nan("");  // a row of -inf has no distribution
+  const float ref = has_out ? out.m : top;
+  const double h = a.hard, z1 = two ? all_s1 : all_s;
   double loss = (1 - h) * a.temperature * a.temperature * kd;
-  if (h > 0) loss += h * (log(z1) - ((double)T::load(z[r.y]) - all.m));
+  if (h > 0) loss += h * (log(z1) - ((double)T::load(z[r.y]) - top));
   loss_rows[row] = (float)loss;
   const double w = (1 - h) * a.temperature;
   st[0] = ref;
-  st[1] = (float)(w * co + (h > 0 && !two ? h * exp((double)ref - all.m) / z1 : 0.0));
-  st[2] = all.m;
-  st[3] = r.any ? (float)(w * mass / all.s) : 0.f;
+  st[1] = (float)(w * co + (h > 0 && !two ? h * exp((double)ref - top) / z1 : 0.0));
+  st[2] = top;
+  st[3] = r.any ? (float)(w * mass / all_s) : 0.f;
   st[4] = h > 0 ? (float)(h / z1) : 0.f;
   st[5] = 1.f;
   const float hi = (float)norm;

@@ -163,14 +163,19 @@ def oracle(z, tv, ti, target, tlse, T, h):
             if rest > 0 and out.any() and z[r][out].amax() > -INF:
                 lo = torch.logsumexp(z[r][out] / T, 0)
                 kd = kd + rest * (math.log(rest) - (lo - lz))
-                err = err + 2 * rest * es(V)
+                # log q_rest = -log(1 + inside / outside): an error of the sum outside moves it by the
+                # share inside only, so a small difference of p and q is not lost in their rest
+                inside = q[~out].sum()
+                err = err + rest * inside * (es(V) + 4 * E)
                 qt = torch.where(out, (z[r] / T - lo).exp(), 0.0)
                 do = (z[r][out].amax() - z[r]).clamp_min(0) / T
                 mass, far = mass + rest, rest * qt
-                # the share of a class outside is one exponential times a difference of two terms
-                eg = eg + times(rest * qt + torch.where(out, q, 0.0), es(V) + 4 * E * (do + 1)) + 2 * E * (rest * qt)
+                # a class outside: one exponential times (q_rest - rest)
+                diff = ((lo - lz).exp() * mass - rest).abs()
+                eg = torch.where(out, times(diff * qt, es(V) + 4 * E * (do + 1)) + qt * inside * (es(V) + 4 * E), eg)
         g = w * (mass * q - far - big)
-        eg = w * (max(1.0, float(mass)) * eg + 4 * E * (mass * q + big))
+        own = torch.zeros(V, dtype=torch.float64).index_fill(0, c, 1.0) if tlse is not None else 1.0
+        eg = w * (max(1.0, float(mass)) * eg + 4 * E * (mass * q * own + big))
         loss[r] = (1 - h) * T * T * kd
         tl[r] = (1 - h) * T * T * err
         if h > 0:
@@ -320,6 +325,19 @@ def test_distill_loss_far_values(dev):
     for T, h in ((1.0, 0.0), (1.0, 0.5), (2.0, 0.5)):
         check_distill(dev, z, tv, ti, y if h else None, lse, T, h)
         check_distill(dev, z, tv, ti, y if h else None, None, T, h)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("V,k,T", [(300, 2, 4.0), (50000, 1, 4.0), (50000, 40, 8.0)])
+def test_distill_loss_small_shares(dev, V, k, T):
+    """Named classes that hold little, a student near its teacher: the loss is a small difference of
+    the shares, and so is the gradient of every class outside."""
+    g = torch.Generator().manual_seed(V)
+    teacher = torch.randn(4, V, generator=g)
+    z = teacher + 0.05 * torch.randn(4, V, generator=g)
+    tv, ti, lse = ops.top_logits(teacher, k, T)
+    check_distill(dev, z, tv, ti, None, lse, T)
+    check_distill(dev, z, tv, ti, None, lse, T, 0.0, "none")
 
 
 @pytest.mark.parametrize("dev", DEVICES)
