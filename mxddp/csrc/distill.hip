@@ -529,7 +529,7 @@ __device__ __forceinline__ void load_entry(const DistillArgs& a, int64_t row, do
 // bound by the row's bytes.  Classes outside the named ones are told by a bit each in LDS, looked at
 // once a piece.  Backward: the same pieces, read again and written; the named classes and the label
 // are written over afterwards by their own threads.
-constexpr int kMaskBits = 1 << 17;  // classes whose bits are in LDS at a time
+constexpr int kMaskWords = 4096;  // a thread's elements of a tile have one: 131,072 classes at a time, 65,536 of fp32
 
 // sums of a row's exponentials at T, and at 1 where the labels need it too, relative to one maximum
 struct Sums {
@@ -566,7 +566,8 @@ __device__ __forceinline__ Sums block_merge(Sums v, float c, float c1, float* re
 template <class T>
 __device__ __forceinline__ Sums row_sums(const DistillArgs& a, const typename T::store_t* z, int begin, int end,
                                          int cls, bool two, uint32_t* mask, float* red) {
-  constexpr int N = Piece<T>::kN, TILE = kT * kU * N;
+  constexpr int N = Piece<T>::kN, TILE = kT * kU * N, kMasked = kMaskWords / kT * TILE;
+  static_assert(kU * N <= 32, "a word has a bit for each of a thread's elements");
   const int tid = threadIdx.x;
   const float c = (float)(kLog2e / a.temperature), c1 = (float)kLog2e;
   const bool tail = a.tlse != nullptr;
@@ -580,8 +581,8 @@ __device__ __forceinline__ Sums row_sums(const DistillArgs& a, const typename T:
     if (cls >= v0 && cls < v0 + n) atomicOr(&mask[word(cls - v0)], 1u << bit(cls - v0));
     __syncthreads();
   };
-  for (int v0 = begin; v0 < end; v0 += kMaskBits) {
-    const int n = min(end - v0, kMaskBits);
+  for (int v0 = begin; v0 < end; v0 += kMasked) {
+    const int n = min(end - v0, kMasked);
     if (tail) set_mask(v0, n);
 #pragma unroll 1
     for (int base = 0; base < n; base += TILE) {
@@ -621,8 +622,8 @@ __device__ __forceinline__ Sums row_sums(const DistillArgs& a, const typename T:
   v = block_merge(v, c, c1, red);
   if (unsettled(v.m, v.s, c) || (two && unsettled(v.m, v.s1, c1))) {
     MaxSum o, o1;
-    for (int v0 = begin; v0 < end; v0 += kMaskBits) {
-      const int n = min(end - v0, kMaskBits);
+    for (int v0 = begin; v0 < end; v0 += kMasked) {
+      const int n = min(end - v0, kMasked);
       if (tail) set_mask(v0, n);
       for (int i = tid; i < n; i += kT) {
         if (tail && (mask[word(i)] >> bit(i) & 1)) continue;
@@ -750,7 +751,7 @@ template <class T>
 __global__ __launch_bounds__(kT, 8) void distill_fwd_k(DistillArgs a, int nseg, int seglen, float* __restrict__ part,
                                                     float* __restrict__ loss_rows) {
   __shared__ RowShared sh;
-  __shared__ uint32_t mask[kMaskBits / 32];
+  __shared__ uint32_t mask[kMaskWords];
   const int64_t row = blockIdx.x / nseg;
   const int seg = blockIdx.x % nseg;
   const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;

@@ -327,6 +327,27 @@ def test_distill_loss_far_values(dev):
         check_distill(dev, z, tv, ti, y if h else None, None, T, h)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [65537, 140001])
+def test_distill_loss_whole_long_rows(cuda, dtype, V):
+    """So many rows that each is one block's: longer ones than the classes whose marks are in LDS at a
+    time.  The teacher's classes spread over the whole row; most rows are left out."""
+    N, k = 520, 40
+    g = torch.Generator().manual_seed(V)
+    z = torch.zeros(N, V, dtype=dtype)
+    rows = [0, 7, N - 1]
+    z[rows] = (2 * torch.randn(3, V, generator=g)).to(dtype)
+    tv = (torch.randn(N, k, generator=g) + 2).to(dtype)
+    ti = torch.randint(V, (N, k), generator=g)
+    ti[rows, 0] = V - 1
+    lse = torch.full((N,), 8.0)
+    y = torch.full((N,), -100)
+    y[rows] = torch.tensor([3, 65536, V - 1])
+    for T, h in ((1.0, 0.0), (2.0, 0.5)):
+        check_distill("cuda", z, tv, ti, y, lse, T, h)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("V,k,T", [(300, 2, 4.0), (50000, 1, 4.0), (50000, 40, 8.0)])
 def test_distill_loss_small_shares(dev, V, k, T):
