@@ -6,6 +6,7 @@
 // the smaller one's last place), says which way.
 // int8_gemm_k: rows of q and rows of w, both contiguous in k, on v_mfma_i32_16x16x64_i8; the sum is a
 // whole number below 2^31, so it is exact in any order.
+#include <algorithm>
 #include <type_traits>
 
 #include "lowp.h"
@@ -487,10 +488,20 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void int8_skinny_k(GemmArgs a, c
 template <class T, int FM, int FN, bool QUANT = false>
 void launch_skinny(GemmArgs a, hipStream_t st, const void* x = nullptr, int64_t ldx = 0) {
   a.tiles_n = cdiv(a.N, 16 * FM);
-  const int64_t blocks = (a.M + 16 * FN - 1) / (16 * FN) * a.tiles_n;
-  MX_CHECK(blocks <= kMaxRows, "linear_int8: too many tiles");
-  MX_LAUNCH((int8_skinny_k<T, FM, FN, QUANT>), dim3((uint32_t)blocks), dim3(64 * kSkinnyWaves), 0, st, a,
-            static_cast<const typename T::store_t*>(x), ldx);
+  // as many tokens a launch as its grid takes
+  const int64_t M = a.M, most = std::max<int64_t>(kMaxRows / a.tiles_n, 1) * 16 * FN;
+  for (int64_t m = 0; m < M; m += most) {
+    a.M = std::min(most, M - m);
+    const int64_t blocks = (a.M + 16 * FN - 1) / (16 * FN) * a.tiles_n;
+    MX_CHECK(blocks <= kMaxRows, "linear_int8: too many tiles");
+    MX_LAUNCH((int8_skinny_k<T, FM, FN, QUANT>), dim3((uint32_t)blocks), dim3(64 * kSkinnyWaves), 0, st, a,
+              static_cast<const typename T::store_t*>(x), ldx);
+    if constexpr (!QUANT) {
+      a.q += a.M * a.ldq;
+      a.xs += a.M;
+    }
+    a.y = static_cast<typename T::store_t*>(a.y) + a.M * a.N;
+  }
 }
 
 }  // namespace

@@ -37,7 +37,8 @@ def _check_temperature(t) -> float:
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     """The k largest logits of each row, in falling order, equal ones by their class.
 
-    ``logits``: [..., V] float32, bfloat16 or float16; 1 <= k <= min(V, 256).  A NaN counts as the
+    ``logits``: [..., V] float32, bfloat16 or float16, at most 8388607 rows and 2^30 classes;
+    1 <= k <= min(V, 256).  A NaN counts as the
     largest value.  ``lse`` is taken at ``temperature`` over all classes (infinite or NaN where the
     largest logit is).  The results carry no gradient."""
     check_float(logits, "top_logits: logits")
@@ -150,7 +151,8 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torc
 
         loss = (1 - hard_weight) T^2 KL(p || q) + hard_weight cross_entropy(logits, target)
 
-    ``logits``: [..., V], the student's, float32, bfloat16 or float16.  ``top_values`` [..., k] (one
+    ``logits``: [..., V], the student's, float32, bfloat16 or float16, at most 8388607 rows and 2^30
+    classes.  ``top_values`` [..., k] (one
     of these types) and ``top_index`` [..., k] (int32 or int64): the teacher's logits for k <= 256
     named classes, as ``top_logits`` gives them.  An entry whose index lies outside [0, V) or whose
     value is -inf is unused; a class named twice has both entries' share.

@@ -22,7 +22,7 @@ def quantize_rows(x: torch.Tensor):
 
     ``scale = max|x| / 127`` (at least 2^-126) and ``q = x / scale`` rounded half to even, exactly.
     A row with an infinity or a NaN has a NaN scale and q = 0.  ``x``: [..., K], float32, bfloat16
-    or float16.  Weights [out, in] give the per-channel scales that ``linear_int8`` takes."""
+    or float16, at most 8388607 rows.  Weights [out, in] give the per-channel scales that ``linear_int8`` takes."""
     check_float(x, "quantize_rows: x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"quantize_rows: x must be [..., K] with K >= 1, got {tuple(x.shape)}")
@@ -62,8 +62,11 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     ``weight``: int8 [N, K], contiguous rows of any stride; ``weight_scale``: float32 [N];
     ``bias``: float32 [N].  ``x``: [..., K] in float32, bfloat16 or float16, or int8 with its
     ``x_scale`` [...] (``quantize_rows``: one quantised input for several layers).  The result has
-    ``out_dtype`` (default: x's type, float32 for an int8 x).  K is at most 131071.  No gradient: an
-    ``x`` that requires one is refused while autograd records."""
+    ``out_dtype`` (default: x's type, float32 for an int8 x).  K is at most 131071, and x has at most
+    8388607 rows.  No gradient: an input that requires one is refused while autograd records.
+
+    Rows of whole 16-byte pieces (K a multiple of 16, or a weight with padded rows as ``Int8Linear``
+    keeps it) take the faster way into the large tiles."""
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear_int8: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
     N, K = weight.shape
@@ -79,8 +82,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         check_float(x, "linear_int8: x")
         if x_scale is not None:
             raise ValueError("linear_int8: x_scale goes with an int8 x")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad() or detach x")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight_scale, bias, x_scale)):
+        raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad() or detach its inputs")
     out_dtype = out_dtype or (torch.float32 if given else x.dtype)
     if out_dtype not in DTYPES:
         raise TypeError(f"linear_int8: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")

@@ -267,6 +267,8 @@ def test_refusals():
         (lambda: ops.linear_int8(x.to(torch.int8), w, ws, x_scale=torch.ones(4).double()), ValueError),
         (lambda: ops.linear_int8(x, w, ws, out_dtype=torch.int8), TypeError),
         (lambda: ops.linear_int8(x.clone().requires_grad_(), w, ws), RuntimeError),
+        (lambda: ops.linear_int8(x, w, ws, b.clone().requires_grad_()), RuntimeError),
+        (lambda: ops.linear_int8(x, w, ws.clone().requires_grad_()), RuntimeError),
         (lambda: ops.linear_int8(torch.zeros(1, 2**17), torch.zeros(2, 2**17, dtype=torch.int8), ws[:2]), ValueError),
         (lambda: ops.linear_int8(x, w, ws.to("meta")), ValueError),
     ]:
