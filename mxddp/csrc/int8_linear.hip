@@ -378,7 +378,7 @@ void launch_gemm(GemmArgs a, bool dw, bool dq, hipStream_t st) {
   a.tiles_m = (int)tm;
   const dim3 grid((uint32_t)(tm * a.tiles_n)), block(64 * WM * WN);
   if (dw && dq) MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, NS, true, true>), grid, block, 0, st, a);
-  else if constexpr (TM * TN <= 128 * 128) {  // a larger tile's registers do not hold a stage as well
+  else if constexpr (TM * TN <= 192 * 256) {  // a larger tile's registers do not hold a stage as well
     if (dq) MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, 2, false, true>), grid, block, 0, st, a);
     else MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, 2, false, false>), grid, block, 0, st, a);
   }
@@ -532,17 +532,23 @@ void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, cons
     return ((uintptr_t)p | (uintptr_t)ld) % 16 == 0 && room >= (K + 15) / 16 * 16;
   };
   const bool dw = whole(w, ldw, w_room), dq = whole(q, ldq, q_room);
-  // A tile kernel's time is its rounds over the machine times a stage's time, measured in us at
-  // K = 4096 and 8192: 64 x 64 0.55 with two blocks a CU; 128 x 128 0.8 with one, 1.1 with two (of half
-  // the stages in LDS); 256 x 256 1.8 with one.  4096^3: 73 us on the largest, 90 on 128 x 128; 512 x
-  // 4096 x 4096: 20 us on the smallest, 25 on 128 x 128.
+  // A tile kernel's time is its rounds over the machine times the time of a stage, in us as measured at
+  // K of 4096 to 8192 (copied straight to LDS; through registers): 64 x 64 with two blocks a CU 0.55
+  // (0.8), 128 x 128 with one and four stages in LDS 0.72, with two and two stages 1.1 (1.27), 192
+  // channels x 256 tokens 1.6 (2.1), 256 x 256 1.8.  So 512 x 4096 x 4096 takes 17 us on the smallest (25
+  // on 128 x 128), 1777 x 5008 x 5008 64 us on 192 x 256 (72 on 256 x 256, 91 on 128 x 128), and 4096^3
+  // 61 us on the largest (82 on 192 x 256).
   const int64_t cu = device_cu_count();
-  auto rounds = [&](int t, int64_t slots) {
-    const int64_t tiles = (M + t - 1) / t * cdiv(N, t);
+  auto rounds = [&](int tn, int tm, int64_t slots) {
+    const int64_t tiles = (M + tm - 1) / tm * cdiv(N, tn);
     return (double)((tiles + slots - 1) / slots);
   };
-  const double c64 = 0.55 * rounds(64, 2 * cu), c128 = 0.8 * rounds(128, cu), c128x2 = 1.1 * rounds(128, 2 * cu);
-  const double c256 = dw && dq ? 1.8 * rounds(256, cu) : 1e30;
+  const bool dma = dw && dq;
+  const double never = 1e30;
+  const double cost[5] = {(dma ? 0.55 : 0.8) * rounds(64, 64, 2 * cu), dma ? 0.72 * rounds(128, 128, cu) : never,
+                          (dma ? 1.1 : 1.27) * rounds(128, 128, 2 * cu), (dma ? 1.6 : 2.1) * rounds(192, 256, cu),
+                          dma ? 1.8 * rounds(256, 256, cu) : never};
+  const int best = (int)(std::min_element(cost, cost + 5) - cost);
   MX_BY_TYPE(ytype, T, {
     // Few tokens: the weight's bytes, and for each block the tokens'.  Twice the channels a block halve
     // the latter, where that leaves a block a CU: 16 tokens of 8192 x 8192 16 us (19 without), of 4096 x
@@ -554,10 +560,10 @@ void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, cons
     } else if (M <= 32) {
       if (wide) launch_skinny<T, 2, 2>(a, st);
       else launch_skinny<T, 1, 2>(a, st);
-    }
-    else if (c64 <= c128 && c64 <= c128x2 && c64 <= c256) launch_gemm<T, 64, 64, 2, 2, 4>(a, dw, dq, st);
-    else if (c128 <= c128x2 && c128 <= c256 && dw && dq) launch_gemm<T, 128, 128, 2, 4, 4>(a, dw, dq, st);
-    else if (c128x2 <= c256) launch_gemm<T, 128, 128, 2, 4, 2>(a, dw, dq, st);
+    } else if (best == 0) launch_gemm<T, 64, 64, 2, 2, 4>(a, dw, dq, st);
+    else if (best == 1) launch_gemm<T, 128, 128, 2, 4, 4>(a, dw, dq, st);
+    else if (best == 2) launch_gemm<T, 128, 128, 2, 4, 2>(a, dw, dq, st);
+    else if (best == 3) launch_gemm<T, 192, 256, 2, 4, 2>(a, dw, dq, st);
     else launch_gemm<T, 256, 256, 2, 4, 2>(a, dw, dq, st);
   });
 }

@@ -129,7 +129,7 @@ def test_linear_int8(dev, M, N, K):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,N", [(2309, 4100), (1000, 4000), (1100, 4100), (520, 3970), (20, 8200), (9, 8197)])
+@pytest.mark.parametrize("M,N", [(2309, 4100), (3999, 4050), (1000, 4000), (1100, 4100), (520, 3970), (20, 8200), (9, 8197)])
 @pytest.mark.parametrize("K", [7, 16, 112, 128, 144, 250, 256, 384, 520, 640, 1008])
 def test_linear_int8_tiles(cuda, M, N, K):
     """Every tile kernel (their choice goes by rounds over the machine), one stage of k to eight, k that
