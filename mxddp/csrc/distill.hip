@@ -61,19 +61,23 @@ struct MaxSum {
 constexpr int kT = 256;
 constexpr int kU = 4;  // pieces of 16 bytes a thread holds: a tile is TB * kU pieces
 
-// 16 bytes at any address, past the caches: a pass reads or writes a row once.  A distillation step of
-// 4096 x 131072 in bf16: 678 us with ordinary accesses, 667 with these loads, 600 with the stores too.
+// 16 bytes at any address.  The forward reads past the caches, what it reads is not read again soon
+// (2048 x 65536 in bf16: 55 us with it, 60 without).  The backward reads through them (4096 x 131072 in
+// bf16: 446 us, 461 with reads past them) and writes past them (the whole step 600 us, 667 with ordinary
+// writes), but only rows of whole cache lines: parts of lines written past the caches cost more (1023 x
+// 50001 in fp16: 53 us, 40 with ordinary writes).
 typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(1)));
 
 // a thread's pieces of the tile at `base` (rows end at `end`); inside the row no lane looks at the end
-template <class T, int TB>
+template <class T, int TB, bool PAST = true>
 __device__ __forceinline__ void load_tile(Piece<T>* x, const typename T::store_t* z, int base, int end) {
   constexpr int N = Piece<T>::kN;
   if (base + TB * kU * N <= end) {
     const typename T::store_t* p = z + base + threadIdx.x * N;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const any16 b = __builtin_nontemporal_load(reinterpret_cast<const any16*>(p + u * TB * N));
+      const any16* q = reinterpret_cast<const any16*>(p + u * TB * N);
+      const any16 b = PAST ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[u].v[j] = b[j];
     }
@@ -852,10 +856,11 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
   // without a share (co = 0) a named class above `ref` must not make a NaN of an overflow
   const float lim = co == 0.f ? 0.f : INFINITY;
   constexpr int TILE = kT * kU * N;
+  const bool lines = ((uintptr_t)(dz + begin) & 127) == 0;
 #pragma unroll 1
   for (int base = begin; base < end; base += TILE) {
     Piece<T> x[kU];
-    load_tile<T, kT>(x, z, base, end);
+    load_tile<T, kT, false>(x, z, base, end);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int i = base + (u * kT + tid) * N;
@@ -870,7 +875,8 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
       if (i + N <= end) {
         any16 w;
         __builtin_memcpy(&w, o, 16);
-        __builtin_nontemporal_store(w, reinterpret_cast<any16*>(dz + i));
+        if (lines) __builtin_nontemporal_store(w, reinterpret_cast<any16*>(dz + i));
+        else *reinterpret_cast<any16*>(dz + i) = w;
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
