@@ -14,6 +14,7 @@
 // their own, so what they hold is never the difference of two near numbers, and a row's exponentials
 // are taken relative to that maximum: none of them overflows.
 #include <algorithm>
+#include <type_traits>
 
 #include "lowp.h"
 #include "ops.h"
@@ -61,11 +62,8 @@ struct MaxSum {
 constexpr int kT = 256;
 constexpr int kU = 4;  // pieces of 16 bytes a thread holds: a tile is TB * kU pieces
 
-// 16 bytes at any address.  The forward reads past the caches, what it reads is not read again soon
-// (2048 x 65536 in bf16: 55 us with it, 60 without).  The backward reads through them (4096 x 131072 in
-// bf16: 446 us, 461 with reads past them) and writes past them (the whole step 600 us, 667 with ordinary
-// writes), but only rows of whole cache lines: parts of lines written past the caches cost more (1023 x
-// 50001 in fp16: 53 us, 40 with ordinary writes).
+// 16 bytes at any address.  The forward and the top logits read past the caches: a row is not read again
+// soon (2048 x 65536 in bf16: 55 us with it, 60 without).
 typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(1)));
 
 // a thread's pieces of the tile at `base` (rows end at `end`); inside the row no lane looks at the end
@@ -828,7 +826,7 @@ __global__ __launch_bounds__(1024) void distill_mean_k(const float* __restrict__
 
 template <class T>
 __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int seglen,
-                                                    const float* __restrict__ dloss, int per_row,
+                                                    const float* __restrict__ dloss, int per_row, int past_caches,
                                                     typename T::store_t* __restrict__ dz) {
   constexpr int N = Piece<T>::kN;
   __shared__ int cls_s[kT];
@@ -856,34 +854,38 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
   // without a share (co = 0) a named class above `ref` must not make a NaN of an overflow
   const float lim = co == 0.f ? 0.f : INFINITY;
   constexpr int TILE = kT * kU * N;
-  const bool lines = ((uintptr_t)(dz + begin) & 127) == 0;
+  // a loop for each kind of access: of two stores under a condition the compiler makes one ordinary one
+  auto sweep = [&](auto past) {
 #pragma unroll 1
-  for (int base = begin; base < end; base += TILE) {
-    Piece<T> x[kU];
-    load_tile<T, kT, false>(x, z, base, end);
+    for (int base = begin; base < end; base += TILE) {
+      Piece<T> x[kU];
+      load_tile<T, kT, past.value>(x, z, base, end);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int i = base + (u * kT + tid) * N;
-      typename T::store_t o[N];
+      for (int u = 0; u < kU; ++u) {
+        const int i = base + (u * kT + tid) * N;
+        typename T::store_t o[N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float v = x[u].get(e);
-        float d = co * fminf(exp2_raw((v - ref) * c), lim);
-        if (two) d += h1 * exp2_raw((v - m) * c1);
-        o[e] = T::store(g * d);
-      }
-      if (i + N <= end) {
-        any16 w;
-        __builtin_memcpy(&w, o, 16);
-        if (lines) __builtin_nontemporal_store(w, reinterpret_cast<any16*>(dz + i));
-        else *reinterpret_cast<any16*>(dz + i) = w;
-      } else {
+        for (int e = 0; e < N; ++e) {
+          const float v = x[u].get(e);
+          float d = co * fminf(exp2_raw((v - ref) * c), lim);
+          if (two) d += h1 * exp2_raw((v - m) * c1);
+          o[e] = T::store(g * d);
+        }
+        if (i + N <= end) {
+          any16 w;
+          __builtin_memcpy(&w, o, 16);
+          if constexpr (past.value) __builtin_nontemporal_store(w, reinterpret_cast<any16*>(dz + i));
+          else *reinterpret_cast<any16*>(dz + i) = w;
+        } else {
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (i + e < end) dz[i + e] = o[e];
+          for (int e = 0; e < N; ++e)
+            if (i + e < end) dz[i + e] = o[e];
+        }
       }
     }
-  }
+  };
+  if (past_caches) sweep(std::true_type{});
+  else sweep(std::false_type{});
   int cls;
   double u;
   load_entry(a, row, inv_t, &cls, &u);
@@ -974,9 +976,16 @@ void distill_bwd(const DistillArgs& a, const float* dloss, bool per_row, void* d
   check_distill(a);
   int nseg = row_segments(a.rows, a.V);
   const int seglen = segment_length(a.V, &nseg);
+  // Past the caches, reads and writes: rows of whole cache lines that the last-level cache of 256 MB does
+  // not hold.  A step (both directions) of 4096 x 131072 in bf16: 599 us, 615 with the writes alone, 667
+  // with ordinary writes.  Other rows the other way round: 1023 x 50001 in fp16 40 us through the caches
+  // and 46 past them, 4096 x 131071 in bf16 489 and 516 (partial lines are joined in the cache).
+  const int64_t row_bytes = (int64_t)a.V * (a.type == kF32 ? 4 : 2);
+  const bool past = ((uintptr_t)dz | (uintptr_t)row_bytes) % 128 == 0 && a.rows * row_bytes >= (256ll << 20);
   if (a.rows > 0)
     MX_BY_TYPE(a.type, T, MX_LAUNCH(distill_bwd_k<T>, dim3((uint32_t)(a.rows * nseg)), dim3(kT), 0, st, a, nseg,
-                                    seglen, dloss, per_row ? 1 : 0, static_cast<typename T::store_t*>(dz)));
+                                    seglen, dloss, per_row ? 1 : 0, past ? 1 : 0,
+                                    static_cast<typename T::store_t*>(dz)));
 }
 
 }  // namespace mx

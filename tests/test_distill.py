@@ -610,6 +610,32 @@ def test_offsets_past_32_bits(cuda):
     assert bool(((dz[-6:].cpu().double() - grad).abs() <= tol).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,N,V", [(torch.bfloat16, 2048, 65536), (torch.float32, 700, 98304), (torch.float16, 1500, 98368)])
+def test_distill_large_gradient(cuda, dtype, N, V):
+    """A gradient of more than 256 MB: the same bits as those of its rows taken in smaller calls, and its
+    last rows against the formula."""
+    k, T, h = 40, 2.0, 0.3
+    g = torch.Generator(device=cuda).manual_seed(23)
+    z = (3 * torch.randn(N, V, generator=g, device=cuda)).to(dtype)
+    tv, ti, lse = ops.top_logits(3 * torch.randn(N, V, generator=g, device=cuda), k, T)
+    y = torch.randint(V, (N,), generator=g, device=cuda)
+
+    def gradient(a, b):
+        zs = z[a:b].detach().requires_grad_()
+        loss = ops.distill_loss(zs, tv[a:b], ti[a:b], y[a:b], lse[a:b], T, h, "sum")
+        return torch.autograd.grad(loss, zs)[0]
+
+    whole = gradient(0, N)
+    for a in list(range(0, N - 512, 512)) + [N - 512]:  # 512 rows: a block to a row, as in the whole
+        assert torch.equal(whole[a:a + 512], gradient(a, a + 512))
+    _, _, grad, _, tg = oracle(z[-3:].cpu(), tv[-3:].cpu(), ti[-3:].cpu(), y[-3:].cpu(), lse[-3:].cpu(), T, h)
+    fi = torch.finfo(dtype)
+    tol = tg + 3 * E * grad.abs()
+    tol = tol + fi.eps / 2 * (grad.abs() + tol) + fi.smallest_normal * fi.eps
+    assert bool(((whole[-3:].cpu().double() - grad).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_teacher_to_student(dev):
     """The operators together: a teacher with int8 layers answers, its top logits are kept, a student
