@@ -254,24 +254,20 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
     for (int j = 0; j < kCopies; ++j) copy(t, buf, j);
   };
   // to registers, and from there to LDS
-  auto load = [&](int t) {
+  constexpr int kPieces = (DW ? 0 : IA) + (DQ ? 0 : IB);
+  auto load = [&](int t, int j) {
     const int at = min(t * 128 + chunk, a.K - 16) - chunk;
-#pragma unroll
-    for (int j = 0; j < (DW ? 0 : IA); ++j) rw[j] = load16(wbase + at + offw[j]);
-#pragma unroll
-    for (int j = 0; j < (DQ ? 0 : IB); ++j) rq[j] = load16(qbase + at + offq[j]);
+    const int i = DW ? j : j - IA;
+    if (!DW && j < IA) rw[j] = load16(wbase + at + offw[j]);
+    else rq[i] = load16(qbase + at + offq[i]);
   };
-  auto put = [&](int t, int buf) {
+  auto put = [&](auto end, int t, int buf, int j) {
     char* st = sm + buf * SB + lane * 16;
-    const int over = t * 128 + 128 > a.K ? t * 128 + chunk + 16 - a.K : 0;
-    auto to = [&](char* p, i32x4 v) {
-      if (t * 128 + 128 > a.K) v = tail16(v, over);
-      *reinterpret_cast<i32x4*>(p) = v;
-    };
-#pragma unroll
-    for (int j = 0; j < (DW ? 0 : IA); ++j) to(st + (wave * IA + j) * 1024, rw[j]);
-#pragma unroll
-    for (int j = 0; j < (DQ ? 0 : IB); ++j) to(st + TM * 128 + (wave * IB + j) * 1024, rq[j]);
+    const int i = DW ? j : j - IA;
+    const bool w = !DW && j < IA;
+    i32x4 v = w ? rw[j] : rq[i];
+    if constexpr (end.value) v = tail16(v, max(t * 128 + chunk + 16 - a.K, 0));
+    *reinterpret_cast<i32x4*>(st + (w ? (wave * IA + j) * 1024 : TM * 128 + (wave * IB + i) * 1024)) = v;
   };
   const int fr = lane & 15, fc = lane >> 4;
   const int rw0 = (wm * FM * 16 + fr) * 128, rq0 = TM * 128 + (wn * FN * 16 + fr) * 128;
@@ -289,19 +285,16 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
     }
   };
   i32x4 acc[FM][FN] = {};
-  // the products of (fw, fq); between them the reads of half a stage to (nw, nq) and the copies of stage t2
-  auto products = [&](auto more, auto copies, const i32x4* fw, const i32x4* fq, int nbuf, int nhalf, i32x4* nw,
-                      i32x4* nq, int t2, int cbuf) {
+  // the products of (fw, fq); between them the reads of half a stage to (nw, nq) and `side`, a share at a time
+  auto products = [&](auto more, const i32x4* fw, const i32x4* fq, int nbuf, int nhalf, i32x4* nw, i32x4* nq,
+                      auto side) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       if constexpr (more.value) {
 #pragma unroll
         for (int r = i * (FM + FN) / FM; r < (i + 1) * (FM + FN) / FM; ++r) read(nbuf, nhalf, r, nw, nq);
       }
-      if constexpr (copies.value) {
-#pragma unroll
-        for (int j = i * kCopies / FM; j < (i + 1) * kCopies / FM; ++j) copy(t2, cbuf, j);
-      }
+      side(i);
 #pragma unroll
       for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fq[j], acc[i][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
@@ -311,9 +304,9 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
   constexpr std::false_type no{};
 
   const int nt = (a.K + 127) / 128;
-  // through registers a stage is loaded behind the barrier before its turn and put in its place in the
-  // middle of the stage before it; the last stage is loaded again rather than under a condition, which
-  // would make the compiler wait for it at once
+  // through registers a stage is loaded in the second half of the last but one before it, and put in its
+  // place in the first half of the one before it; the last stage is loaded again rather than under a
+  // condition, which would make the compiler wait for it at once
   constexpr bool kDma = DW && DQ;
   constexpr int kAhead = kDma ? NS : 2;
   if constexpr (kDma) {
@@ -324,36 +317,51 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
     else wait_vm<0>();
   } else {
     fetch(0, 0);
-    load(0);
-    put(0, 0);
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) load(0, j);
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) put(yes, 0, 0, j);
     wait_vm<0>();
     if (nt > 1) fetch(1, 1);
-    load(min(1, nt - 1));
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) load(min(1, nt - 1), j);
   }
   lds_barrier();
   i32x4 w0[FM], q0[FN], w1[FM], q1[FN];
 #pragma unroll
   for (int r = 0; r < FM + FN; ++r) read(0, 0, r, w0, q0);
   int buf = 0;
-  // a stage with another behind it, with or without one to copy
+  // a stage with another behind it, with or without one to copy (without: the other is the last)
   auto stage = [&](auto copies, int t) {
     const int next = buf + 1 == NS ? 0 : buf + 1;
-    products(yes, no, w0, q0, buf, 1, w1, q1, 0, 0);
-    if constexpr (!kDma) put(t + 1, next);
+    products(yes, w0, q0, buf, 1, w1, q1, [&](int i) {
+#pragma unroll
+      for (int j = i * kPieces / FM; j < (i + 1) * kPieces / FM; ++j) {
+        if constexpr (copies.value) put(no, t + 1, next, j);
+        else put(yes, t + 1, next, j);
+      }
+    });
     // stage t + 1 has landed; up to NS - 2 later ones are under way
     wait_vm<kDma && copies.value ? (NS - 2) * (IA + IB) : 0>();
     lds_barrier();
-    if constexpr (!kDma) load(min(t + 2, nt - 1));
-    products(yes, copies, w1, q1, next, 0, w0, q0, t + kAhead, buf);
+    products(yes, w1, q1, next, 0, w0, q0, [&](int i) {
+      if constexpr (copies.value) {
+#pragma unroll
+        for (int j = i * kCopies / FM; j < (i + 1) * kCopies / FM; ++j) copy(t + kAhead, buf, j);
+      }
+#pragma unroll
+      for (int j = i * kPieces / FM; j < (i + 1) * kPieces / FM; ++j) load(min(t + 2, nt - 1), j);
+    });
     buf = next;
   };
+  auto nothing = [](int) {};
   int t = 0;
   for (; t + kAhead < nt; ++t) stage(yes, t);
   for (; t + 1 < nt; ++t) stage(no, t);
   clear(t, 0, q0);
-  products(yes, no, w0, q0, buf, 1, w1, q1, 0, 0);
+  products(yes, w0, q0, buf, 1, w1, q1, nothing);
   clear(t, 1, q1);
-  products(no, no, w1, q1, 0, 0, w0, q0, 0, 0);
+  products(no, w1, q1, 0, 0, w0, q0, nothing);
   float xs[FN];
 #pragma unroll
   for (int j = 0; j < FN; ++j) xs[j] = a.xs[min<int64_t>(m0 + (wn * FN + j) * 16 + fr, a.M - 1)];
