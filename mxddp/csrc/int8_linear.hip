@@ -203,13 +203,17 @@ __device__ __forceinline__ void wait_vm() {
 // TM channels x TN tokens per block of WM x WN waves, 128 k a stage, NS stages in LDS.  A stage's rows
 // are 128 bytes, a row's 16-byte pieces XOR-permuted by its number, so the fragments' reads (16 rows at
 // one piece) spread over all banks.  DW, DQ: the channels' and the tokens' rows come straight from
-// global memory (rows of whole, aligned pieces); else through registers (any alignment and K >= 16).  Channels are the matrix instruction's rows: a lane ends with four of them for one
-// token.
+// global memory (rows of whole, aligned pieces); else through registers (any alignment and K >= 16).
+// Channels are the matrix instruction's rows: a lane ends with four of them for one token.
 // The fragments of one half stage are read while the other half's are multiplied.  The barrier stands
 // in the middle of a stage, where its second half is in registers: its buffer is free for stage
-// t + NS there, and the first half of stage t + 1 is read behind it.  Reads and copies are issued one by
-// one between the matrix instructions: a copy of 1 KB keeps its wave from issuing for 16 cycles and
-// more, and all of a stage's in a row leave the matrix units idle for half a stage.
+// t + NS there, and the first half of stage t + 1 is read behind it.  Reads, copies, loads and writes are
+// issued one by one between the matrix instructions: a copy of 1 KB keeps its wave from issuing for 16
+// cycles and more, and all of a stage's in a row leave the matrix units idle for half a stage (8192^3
+// 447 us without it; 1777 x 5000 x 5000, whose rows go through registers, 84).
+// Bound by the matrix units and their operands' way out of LDS: 8192^3 400 to 480 us by the card's clock,
+// 2.3 to 2.75 POP/s, 60% of what the instruction alone reaches on such values; 1777 x 5000 x 5000 66 us,
+// 1.35 POP/s (three quarters of the CUs have a tile).
 template <class T, int TM, int TN, int WM, int WN, int NS, bool DW, bool DQ>
 __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_k(GemmArgs a) {
   constexpr int NW = WM * WN, FM = TM / WM / 16, FN = TN / WN / 16;
@@ -386,10 +390,8 @@ void launch_gemm(GemmArgs a, bool dw, bool dq, hipStream_t st) {
   a.tiles_m = (int)tm;
   const dim3 grid((uint32_t)(tm * a.tiles_n)), block(64 * WM * WN);
   if (dw && dq) MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, NS, true, true>), grid, block, 0, st, a);
-  else if constexpr (TM * TN <= 192 * 256) {  // a larger tile's registers do not hold a stage as well
-    if (dq) MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, 2, false, true>), grid, block, 0, st, a);
-    else MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, 2, false, false>), grid, block, 0, st, a);
-  }
+  else if (dq) MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, 2, false, true>), grid, block, 0, st, a);
+  else MX_LAUNCH((int8_gemm_k<T, TM, TN, WM, WN, 2, false, false>), grid, block, 0, st, a);
 }
 
 // Few tokens: bound by the weight's bytes.  A block of eight waves takes 16 FM channels and all of up
@@ -541,21 +543,22 @@ void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, cons
   };
   const bool dw = whole(w, ldw, w_room), dq = whole(q, ldq, q_room);
   // A tile kernel's time is its rounds over the machine times the time of a stage, in us as measured at
-  // K of 4096 to 8192 (copied straight to LDS; through registers): 64 x 64 with two blocks a CU 0.55
-  // (0.8), 128 x 128 with one and four stages in LDS 0.72, with two and two stages 1.1 (1.27), 192
-  // channels x 256 tokens 1.6 (2.1), 256 x 256 1.8.  So 512 x 4096 x 4096 takes 17 us on the smallest (25
-  // on 128 x 128), 1777 x 5008 x 5008 64 us on 192 x 256 (72 on 256 x 256, 91 on 128 x 128), and 4096^3
-  // 61 us on the largest (82 on 192 x 256).
+  // K of 4096 to 8192 (copied straight to LDS; through registers, between rows of 16 bytes and odd ones):
+  // 64 x 64 with two blocks a CU 0.55 (0.8), 128 x 128 with one and four stages in LDS 0.72, with two and
+  // two stages 1.1 (1.45), 192 channels x 256 tokens 1.6 (1.8), 256 x 256 1.8 (2.35).  So 512 x 4096 x
+  // 4096 takes 17 us on the smallest (25 on 128 x 128), 1777 x 5008 x 5008 60 us on 192 x 256 (69 on 256 x
+  // 256, 87 on 128 x 128), and 4096^3 60 us on the largest (81 on 192 x 256); of odd rows 1024 x 4096 x
+  // 4095 42 us on 128 x 128 (63 on 64 x 64 and on 192 x 256), 4096 x 4096 x 4095 83 us on the largest (122
+  // on 128 x 128 and on 192 x 256).
   const int64_t cu = device_cu_count();
   auto rounds = [&](int tn, int tm, int64_t slots) {
     const int64_t tiles = (M + tm - 1) / tm * cdiv(N, tn);
     return (double)((tiles + slots - 1) / slots);
   };
   const bool dma = dw && dq;
-  const double never = 1e30;
-  const double cost[5] = {(dma ? 0.55 : 0.8) * rounds(64, 64, 2 * cu), dma ? 0.72 * rounds(128, 128, cu) : never,
-                          (dma ? 1.1 : 1.27) * rounds(128, 128, 2 * cu), (dma ? 1.6 : 2.1) * rounds(192, 256, cu),
-                          dma ? 1.8 * rounds(256, 256, cu) : never};
+  const double cost[5] = {(dma ? 0.55 : 0.8) * rounds(64, 64, 2 * cu), dma ? 0.72 * rounds(128, 128, cu) : 1e30,
+                          (dma ? 1.1 : 1.45) * rounds(128, 128, 2 * cu), (dma ? 1.6 : 1.8) * rounds(192, 256, cu),
+                          (dma ? 1.8 : 2.35) * rounds(256, 256, cu)};
   const int best = (int)(std::min_element(cost, cost + 5) - cost);
   MX_BY_TYPE(ytype, T, {
     // Few tokens: the weight's bytes, and for each block the tokens'.  Twice the channels a block halve
