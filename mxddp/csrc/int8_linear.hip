@@ -131,6 +131,31 @@ __device__ __forceinline__ i32x4 load16(const int8_t* p) {
   return i32x4{(int)b.v[0], (int)b.v[1], (int)b.v[2], (int)b.v[3]};
 }
 
+// The 16 bytes at an address: at a multiple of 4 as they are, else from the five words that hold them
+// (a word with a byte of a tensor lies in its allocation).  24 tokens of 8192 x 8191: 32 us, 60 with one
+// read of 16 bytes at an odd address.
+template <bool ODD>
+struct Raw16 {
+  i32x4 v;
+  int more;
+  __device__ __forceinline__ void load(const int8_t* p) {
+    if constexpr (!ODD) {
+      v = load16(p);
+    } else {
+      const uint32_t odd = (uint32_t)(uintptr_t)p & 3;
+      const int8_t* q = p - odd;
+      v = load16(q);
+      more = *reinterpret_cast<const int*>(q + (odd ? 16 : 12));
+    }
+  }
+  __device__ __forceinline__ i32x4 get(const int8_t* p) const {  // p: where it was loaded
+    if constexpr (!ODD) return v;
+    const uint32_t odd = (uint32_t)(uintptr_t)p & 3;
+    return i32x4{(int)__builtin_amdgcn_alignbyte(v[1], v[0], odd), (int)__builtin_amdgcn_alignbyte(v[2], v[1], odd),
+                 (int)__builtin_amdgcn_alignbyte(v[3], v[2], odd), (int)__builtin_amdgcn_alignbyte(more, v[3], odd)};
+  }
+};
+
 // A piece that reaches `over` bytes behind the end of a row was read that much before its place, at
 // the row's last 16 bytes: move it there, with zeros behind the end.
 __device__ __forceinline__ i32x4 tail16(i32x4 v, int over) {
@@ -398,11 +423,16 @@ void launch_gemm(GemmArgs a, bool dw, bool dq, hipStream_t st) {
 // to 16 FN tokens; each wave streams an eighth of k from global memory straight into the matrix
 // instruction's operands (a lane has 16 bytes of one channel, 64 bytes of it lie in one instruction)
 // and the sums, whole numbers, are added in LDS.  The tokens' rows are small and come from the caches.
+// Left to itself the compiler waits for each product's operands soon after their loads.  ODD: rows of no
+// alignment are read word by word.  With weights that no cache holds 1 x 8192 x 8192 takes 15 us (4.3
+// TB/s), 24 tokens of it 20 us (3.3 TB/s: the blocks read as many bytes of the tokens as of the weight;
+// 26 without the order of the loads, 23 with groups of four units, which take more than the nearest cache
+// holds).
 // QUANT: each block quantises the tokens for itself, to LDS: up to kQuantMax values cost it less than
-// a launch before this one (one token of 4096: 7 us with it, 12 without).
+// a launch before this one (one token of 4096 x 4096: 7 us with it, 12 without).
 constexpr int kSkinnyWaves = 8, kQuantMax = 16384;
 
-template <class T, int FM, int FN, bool QUANT>
+template <class T, int FM, int FN, bool ODD, bool QUANT>
 __global__ __launch_bounds__(64 * kSkinnyWaves) void int8_skinny_k(GemmArgs a, const typename T::store_t* x,
                                                                    int64_t ldx) {
   __shared__ i32x4 part[kSkinnyWaves][FM * FN][64];
@@ -443,36 +473,85 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void int8_skinny_k(GemmArgs a, c
 #pragma unroll
   for (int j = 0; j < FN; ++j) pq[j] = a.q + min<int64_t>(m0 + 16 * j + fr, a.M - 1) * a.ldq + 16 * fc;
   i32x4 acc[FM][FN] = {};
-  const int units = (a.K + 63) / 64, whole = a.K / 64;
-  const int u0 = (int)((int64_t)units * wave / kSkinnyWaves), u1 = (int)((int64_t)units * (wave + 1) / kSkinnyWaves);
-  constexpr int U = 8 / FN < 2 ? 2 : 8 / FN;  // units in flight
-  int u = u0;
-  for (; u + U <= min(u1, whole); u += U) {
-    i32x4 fw[U][FM], fq[U][FN];
+  // a wave has groups of U units of 64 k, one after the other: with two a group takes a row's whole cache
+  // lines, and one group is under way while the other is multiplied
+  constexpr int U = 2;
+  const int groups = ((a.K + 63) / 64 + U - 1) / U, each = (groups + kSkinnyWaves - 1) / kSkinnyWaves;
+  struct Group {
+    Raw16<ODD> w[U][FM], q[U][FN];
+  };
+  // a piece that reaches behind the end of k is read at the row's last 16 bytes
+  auto at = [&](int g, int s) { return min(64 * (g * U + s) + 16 * fc, a.K - 16) - 16 * fc; };
+  auto fetch = [&](Group& r, int g) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int s = 0; s < U; ++s) r.w[s][i].load(pw[i] + at(g, s));
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int s = 0; s < U; ++s) {
+        if constexpr (QUANT) r.q[s][j].v = *reinterpret_cast<const i32x4*>(ql + min(64 * (g * U + s), pitch - 80));
+        else r.q[s][j].load(pq[j] + at(g, s));
+      }
+    __builtin_amdgcn_sched_barrier(0);  // all of them under way before the group before it is waited for
+  };
+  auto use = [&](auto end, const Group& r, int g) {
 #pragma unroll
     for (int s = 0; s < U; ++s) {
+      const int over = max(64 * (g * U + s) + 16 * fc + 16 - a.K, 0);
+      i32x4 fw[FM], fq[FN];
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fw[s][i] = load16(pw[i] + 64 * (u + s));
+      for (int i = 0; i < FM; ++i) {
+        fw[i] = r.w[s][i].get(pw[i] + at(g, s));
+        if constexpr (end.value) fw[i] = tail16(fw[i], over);
+      }
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
-        fq[s][j] = QUANT ? *reinterpret_cast<const i32x4*>(ql + 64 * (u + s)) : load16(pq[j] + 64 * (u + s));
-    }
-#pragma unroll
-    for (int s = 0; s < U; ++s)
+      for (int j = 0; j < FN; ++j) {
+        fq[j] = QUANT ? r.q[s][j].v : r.q[s][j].get(pq[j] + at(g, s));
+        if constexpr (end.value && !QUANT) fq[j] = tail16(fq[j], over);
+      }
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[s][i], fq[s][j], acc[i][j], 0, 0, 0);
-  }
-  for (; u < u1; ++u) {  // what is left, the ragged end of k among it
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fq[j], acc[i][j], 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  auto use_last = [&](const Group& r, int g) {
+    if ((g + 1) * U * 64 <= a.K) use(no, r, g);
+    else use(yes, r, g);
+  };
+  if (a.K >= 16) {
+    int g = wave * each;
+    const int last = min(groups, g + each);
+    Group r0, r1;
+    if (g < last) {
+      fetch(r0, g);
+      for (; g + 2 < last; g += 2) {
+        fetch(r1, g + 1);
+        use(no, r0, g);
+        fetch(r0, g + 2);
+        use(no, r1, g + 1);
+      }
+      if (g + 1 < last) {
+        fetch(r1, g + 1);
+        use(no, r0, g);
+        use_last(r1, g + 1);
+      } else {
+        use_last(r0, g);
+      }
+    }
+  } else if (wave == 0) {
     i32x4 fw[FM], fq[FN];
 #pragma unroll
-    for (int i = 0; i < FM; ++i) fw[i] = row16(pw[i] - 16 * fc, true, 64 * u + 16 * fc, a.K);
+    for (int i = 0; i < FM; ++i) fw[i] = row16(pw[i] - 16 * fc, true, 16 * fc, a.K);
 #pragma unroll
     for (int j = 0; j < FN; ++j)
-      fq[j] = QUANT ? *reinterpret_cast<const i32x4*>(ql + 64 * u)
-                    : row16(pq[j] - 16 * fc, true, 64 * u + 16 * fc, a.K);
+      fq[j] = QUANT ? *reinterpret_cast<const i32x4*>(ql) : row16(pq[j] - 16 * fc, true, 16 * fc, a.K);
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -504,8 +583,12 @@ void launch_skinny(GemmArgs a, hipStream_t st, const void* x = nullptr, int64_t 
     a.M = std::min(most, M - m);
     const int64_t blocks = (a.M + 16 * FN - 1) / (16 * FN) * a.tiles_n;
     MX_CHECK(blocks <= kMaxRows, "linear_int8: too many tiles");
-    MX_LAUNCH((int8_skinny_k<T, FM, FN, QUANT>), dim3((uint32_t)blocks), dim3(64 * kSkinnyWaves), 0, st, a,
-              static_cast<const typename T::store_t*>(x), ldx);
+    const dim3 grid((uint32_t)blocks), block(64 * kSkinnyWaves);
+    const auto* xt = static_cast<const typename T::store_t*>(x);
+    auto aligned = [&](const int8_t* p, int64_t ld) { return ((uintptr_t)p | (uintptr_t)ld | (uintptr_t)a.K) % 4 == 0; };
+    const bool odd = !aligned(a.w, a.ldw) || (!QUANT && !aligned(a.q, a.ldq));
+    if (odd) MX_LAUNCH((int8_skinny_k<T, FM, FN, true, QUANT>), grid, block, 0, st, a, xt, ldx);
+    else MX_LAUNCH((int8_skinny_k<T, FM, FN, false, QUANT>), grid, block, 0, st, a, xt, ldx);
     if constexpr (!QUANT) {
       a.q += a.M * a.ldq;
       a.xs += a.M;
@@ -562,8 +645,9 @@ void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, cons
   const int best = (int)(std::min_element(cost, cost + 5) - cost);
   MX_BY_TYPE(ytype, T, {
     // Few tokens: the weight's bytes, and for each block the tokens'.  Twice the channels a block halve
-    // the latter, where that leaves a block a CU: 16 tokens of 8192 x 8192 16 us (19 without), of 4096 x
-    // 4096 9 us (7 without); 32 tokens of 4096 x 4096 9 us, on tiles 19.
+    // the latter, where that leaves a block a CU: 16 tokens of 8192 x 8192 19 us (21 without), of 4096 x
+    // 4096 9.0 us (7.4 without); 32 tokens of 32000 x 4096 42 us (55 without), of 4096 x 4096 9 us, on
+    // tiles 19.
     const bool wide = M > 8 && N >= 32 * cu;
     if (M <= 16 || K < 16) {
       if (wide) launch_skinny<T, 2, 1>(a, st);

@@ -154,6 +154,32 @@ def test_linear_int8_tiles(cuda, M, N, K):
     assert bool(((y.double() - want).abs() <= tol).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("off,ld,K", [(1, 1008, 1001), (3, 1002, 1000), (2, 130, 130), (5, 77, 70), (1, 16, 16),
+                                      (4, 524, 516), (7, 4100, 4099), (15, 5001, 5000)])
+@pytest.mark.parametrize("M,N", [(1, 300), (3, 8200), (12, 8200), (20, 333), (24, 8200), (100, 200), (700, 530)])
+def test_linear_int8_views(cuda, off, ld, K, M, N):
+    """Weights and int8 tokens that begin at any address, rows of any stride, storage that ends with the
+    last row; tokens of a float type as well."""
+    g = torch.Generator(device=cuda).manual_seed(off + M)
+
+    def view(rows):
+        flat = torch.randint(-127, 128, (off + (rows - 1) * ld + K,), generator=g, dtype=torch.int8, device=cuda)
+        return flat.as_strided((rows, K), (ld, 1), off)
+
+    w, q = view(N), view(M)
+    s, ws = torch.rand(M, generator=g, device=cuda), torch.rand(N, generator=g, device=cuda) * 1e-3
+    prod = (q.double() @ w.double().t().contiguous()) * s.double()[:, None] * ws.double()
+    y = ops.linear_int8(q, w, ws, x_scale=s)
+    assert bool(((y.double() - prod).abs() <= 4.02 * E * prod.abs()).all())
+    x = q.float()
+    x[:, K // 3] = -127
+    prod = (x.double() @ w.double().t().contiguous()) * 2.0**-5 * ws.double()
+    y = ops.linear_int8((x * 2.0**-5).to(torch.float16), w, ws, out_dtype=torch.float16).double()
+    tol = 3.01 * E * prod.abs() + 2.0**-11 * 1.001 * prod.abs() + 2.0**-25
+    assert bool(((y - prod).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("M,N,K", [(1, 300, 1024), (5, 77, 96), (5, 77, 99), (70, 200, 1000), (300, 300, 512)])
 @pytest.mark.parametrize("out", TYPES)
