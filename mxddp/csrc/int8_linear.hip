@@ -648,13 +648,15 @@ void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, cons
     // Few tokens: the weight's bytes, and for each block the tokens'.  Twice the channels a block halve
     // the latter, where that leaves a block a CU: 16 tokens of 8192 x 8192 19 us (21 without), of 4096 x
     // 4096 9.0 us (7.4 without); 32 tokens of 32000 x 4096 42 us (55 without), of 4096 x 4096 9 us, on
-    // tiles 19.
+    // tiles 19.  Four times where that leaves one: 32 tokens of 16384 x 8192 34 us (38 with twice), of 32000
+    // x 4095 49 us (58).  Up to 16 tokens it changes nothing.
     const bool wide = M > 8 && N >= 32 * cu;
     if (M <= 16 || K < 16) {
       if (wide) launch_skinny<T, 2, 1>(a, st);
       else launch_skinny<T, 1, 1>(a, st);
     } else if (M <= 32) {
-      if (wide) launch_skinny<T, 2, 2>(a, st);
+      if (N >= 64 * cu) launch_skinny<T, 4, 2>(a, st);
+      else if (wide) launch_skinny<T, 2, 2>(a, st);
       else launch_skinny<T, 1, 2>(a, st);
     } else if (best == 0) launch_gemm<T, 64, 64, 2, 2, 4>(a, dw, dq, st);
     else if (best == 1) launch_gemm<T, 128, 128, 2, 4, 4>(a, dw, dq, st);

@@ -155,6 +155,20 @@ def test_linear_int8_tiles(cuda, M, N, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [17, 24, 32])
+@pytest.mark.parametrize("N,K", [(16384, 128), (16400, 520), (16385, 1001), (20001, 64), (16384, 16), (16399, 7), (32000, 1100)])
+def test_linear_int8_wide(cuda, M, N, K):
+    """Few tokens of very wide layers."""
+    g = torch.Generator(device=cuda).manual_seed(M + N)
+    q = torch.randint(-127, 128, (M, K), generator=g, dtype=torch.int8, device=cuda)
+    w = torch.randint(-127, 128, (N, K), generator=g, dtype=torch.int8, device=cuda)
+    s, ws = torch.rand(M, generator=g, device=cuda), torch.rand(N, generator=g, device=cuda) * 1e-3
+    prod = (q.double() @ w.double().t().contiguous()) * s.double()[:, None] * ws.double()
+    y = ops.linear_int8(q, w, ws, x_scale=s)
+    assert bool(((y.double() - prod).abs() <= 4.02 * E * prod.abs()).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("off,ld,K", [(1, 1008, 1001), (3, 1002, 1000), (2, 130, 130), (5, 77, 70), (1, 16, 16),
                                       (4, 524, 516), (7, 4100, 4099), (15, 5001, 5000)])
 @pytest.mark.parametrize("M,N", [(1, 300), (3, 8200), (12, 8200), (20, 333), (24, 8200), (100, 200), (700, 530)])
