@@ -30,27 +30,20 @@ __device__ __forceinline__ int quant1(float x, float s, float inv) {
   return (int)q;
 }
 
-// A row's scale from its largest magnitude's bits (a thread's in, the block's out).  Infinities and NaN
-// are above every number.
+// A row's scale from its largest magnitude's bits.  Infinities and NaN are above every number.
 struct RowScale {
   float s, inv;
   bool ok;
+  __device__ __forceinline__ explicit RowScale(uint32_t top) {
+    ok = top < 0x7f800000u;
+    s = ok ? fmaxf(__uint_as_float(top) / 127.f, kTiny) : __builtin_nanf("");
+    inv = 1.f / s;
+  }
 };
-template <int TB>
-__device__ __forceinline__ RowScale row_scale(uint32_t top, uint32_t* red) {
+__device__ __forceinline__ uint32_t wave_max(uint32_t top) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-  if constexpr (TB > 64) {
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < TB / 64; ++w) top = max(top, red[w]);
-  }
-  RowScale r;
-  r.ok = top < 0x7f800000u;
-  r.s = r.ok ? fmaxf(__uint_as_float(top) / 127.f, kTiny) : __builtin_nanf("");
-  r.inv = 1.f / r.s;
-  return r;
+  return top;
 }
 
 template <class T>
@@ -89,7 +82,14 @@ __global__ __launch_bounds__(TB) void quantize_rows_k(const typename T::store_t*
 #pragma unroll
       for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(p[u].get(e)) & 0x7fffffffu);
   }
-  const RowScale sc = row_scale<TB>(top, red);
+  top = wave_max(top);
+  if constexpr (TB > 64) {
+    if ((tid & 63) == 0) red[tid >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TB / 64; ++w) top = max(top, red[w]);
+  }
+  const RowScale sc(top);
   if (tid == 0) scale[row] = sc.s;
   for (int k0 = 0; k0 < K; k0 += TILE) {
 #pragma unroll
@@ -430,7 +430,8 @@ void launch_gemm(GemmArgs a, bool dw, bool dq, hipStream_t st) {
 // 26 without the order of the loads, 23 with groups of four units, which take more than the nearest cache
 // holds).
 // QUANT: each block quantises the tokens for itself, to LDS: up to kQuantMax values cost it less than
-// a launch before this one (one token of 4096 x 4096: 7 us with it, 12 without).
+// a launch before this one (one token of 4096 x 4096: 6.6 us with it, 10 without; 16 of 4096 x 1024: 7.5
+// and 8.4), with the waves shared out among the tokens (21 us one token after the other).
 constexpr int kSkinnyWaves = 8, kQuantMax = 16384;
 
 template <class T, int FM, int FN, bool ODD, bool QUANT>
@@ -443,24 +444,34 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void int8_skinny_k(GemmArgs a, c
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fc = lane >> 4;
   const int pitch = (a.K + 63) / 64 * 64 + 16;  // of a token's row in LDS
   if constexpr (QUANT) {
-    constexpr int N = Piece<T>::kN, TB = 64 * kSkinnyWaves;
-    for (int m = 0; m < (int)a.M; ++m) {
-      const typename T::store_t* xr = x + m * ldx;
+    constexpr int N = Piece<T>::kN;
+    // waves of a token; 8 / per tokens at a time
+    const int M = (int)a.M, per = M > 4 ? 1 : M > 2 ? 2 : M > 1 ? 4 : 8;
+    const int first = wave / per * per, at = ((wave - first) * 64 + lane) * N;
+    for (int m0 = 0; m0 < M; m0 += kSkinnyWaves / per) {
+      const int m = m0 + wave / per, K = m < M ? a.K : 0;
+      const typename T::store_t* xr = x + (int64_t)min(m, M - 1) * ldx;
       uint32_t top = 0;
-      for (int k = tid * N; k < a.K; k += TB * N) {
+      for (int k = at; k < K; k += per * 64 * N) {
         Piece<T> p;
-        p.load(xr, k, a.K, 0);
+        p.load(xr, k, K, 0);
 #pragma unroll
         for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(p.get(e)) & 0x7fffffffu);
       }
-      const RowScale sc = row_scale<TB>(top, top_s);
-      if (tid == 0) xs_s[m] = sc.s;
-      for (int k = tid * N; k < pitch - 16; k += TB * N) {
-        Piece<T> p;
-        p.load(xr, k, a.K, 0);  // zeros behind the end
-        uint32_t w[N / 4];
-        quant_piece<T>(p, sc, w);
-        __builtin_memcpy(qs + m * pitch + k, w, N);
+      top = wave_max(top);
+      if (lane == 0) top_s[wave] = top;
+      __syncthreads();
+      for (int w = 0; w < per; ++w) top = max(top, top_s[first + w]);
+      const RowScale sc(top);
+      if (m < M) {
+        if (wave == first && lane == 0) xs_s[m] = sc.s;
+        for (int k = at; k < pitch - 16; k += per * 64 * N) {
+          Piece<T> p;
+          p.load(xr, k, K, 0);  // zeros behind the end
+          uint32_t w[N / 4];
+          quant_piece<T>(p, sc, w);
+          __builtin_memcpy(qs + m * pitch + k, w, N);
+        }
       }
       __syncthreads();
     }

@@ -5,6 +5,8 @@ The quantised values have one right answer each (the exact quotient, rounded hal
 are compared bit for bit.  A product's sum is a whole number; what is left are the roundings of the
 epilogue: the sum to fp32, two scales, the bias, and the result's type, each by half a step.
 """
+import math
+
 import pytest
 import torch
 
@@ -152,6 +154,26 @@ def test_linear_int8_tiles(cuda, M, N, K):
     want = prod + b.double()
     tol = 4.02 * E * prod.abs() + 1.01 * E * (b.double().abs() + want.abs())
     assert bool(((y.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M", range(1, 18))
+@pytest.mark.parametrize("K", [9, 64, 961, 1000, 2040])
+def test_linear_int8_few_tokens(dev, M, K):
+    """Every number of tokens up to 17 of a float type, rows of different sizes of values, one of zeros and
+    one that is not finite."""
+    dtype = TYPES[M % 3]
+    x, w, ws, b = make(M, 70, K, dtype, M * 31 + K)
+    x = x * torch.logspace(-2, 2, M).to(dtype)[:, None]
+    x[M // 2] = 0
+    bad = M - 1 if M > 2 else -1
+    q, s = oracle_quantize(x)
+    if bad > 0:
+        x[bad, K // 2] = math.inf
+    y = ops.linear_int8(x.to(dev), w.to(dev), ws.to(dev), b.to(dev), out_dtype=torch.float32 if K == 64 else None)
+    good = [m for m in range(M) if m != bad]
+    check_linear(y[good], q[good], s[good], w, ws, b, False)
+    assert bad < 0 or bool(torch.isnan(y[bad]).all())
 
 
 @pytest.mark.gpu
