@@ -253,8 +253,7 @@ def _plain_distill(state, case):
         has = (rest > 0) & (log_out > -math.inf)
         kd = kd + torch.where(has, rest * (rest.log() - (log_out - logz)), 0.0)[:, 0]
         share = torch.where(has, rest.log() - log_out, -math.inf).float()
-        mass = p.sum(1, keepdim=True) + torch.where(has, rest, 0.0)
-        grad = grad * mass.float() - torch.where(inside, 0.0, (z / t + share).exp())
+        grad = grad - torch.where(inside, 0.0, (z / t + share).exp())
     else:
         # a row that the teacher says nothing about has no such term
         grad = grad * used.any(1, keepdim=True)
