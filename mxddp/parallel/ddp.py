@@ -7,8 +7,8 @@ Same contract as ``torch.nn.parallel.DistributedDataParallel`` as the reference 
 2. gradients are all-reduced and AVERAGED over ranks every backward, bucketed in reverse
    parameter order (first bucket 1 MB, then 25 MB caps), launched asynchronously as each
    bucket fills so communication overlaps the rest of backward;
-3. floating buffers (BN running stats) are broadcast from rank 0 before every forward
-   (``broadcast_buffers=True``);
+3. floating buffers (BN running stats) and integer ones (an 8-bit layer's weight; not the
+   counters) are broadcast from rank 0 before every forward (``broadcast_buffers=True``);
 4. ``.module`` is the wrapped model, so ``ddp.module.state_dict()`` has no ``module.``
    prefix (checkpoint layout, pytorch/distributed_data_parallel.py:109-113).
 
@@ -32,7 +32,7 @@ import torch.nn as nn
 from .. import native
 from . import comm as _comm
 from . import graphed as _graphed
-from .flat import FlatParams, flatten_buffers
+from .flat import FlatParams, flatten_buffers, flatten_integer_buffers, integer_counters
 
 
 def assign_buckets(numels: list[int], offsets: list[int], total: int, bucket_cap_mb: float = 25.0,
@@ -73,7 +73,9 @@ class DistributedDataParallel(nn.Module):
         self.device = next(module.parameters()).device
         self.flat = FlatParams(module, self.device)
         self.flat_buffers = flatten_buffers(module, self.device) if broadcast_buffers else None
-        self.broadcast_buffers = broadcast_buffers and self.flat_buffers is not None
+        self.flat_bytes = flatten_integer_buffers(module, self.device) if broadcast_buffers else None
+        self.broadcast_buffers = broadcast_buffers and not (self.flat_buffers is None and self.flat_bytes is None)
+        self._counters = integer_counters(module) if broadcast_buffers else []
         numels = [p.numel() for p in self.flat.params]
         self.buckets, self.param_bucket = assign_buckets(numels, self.flat.offsets, self.flat.numel, bucket_cap_mb,
                                                          first_bucket_cap_mb)
@@ -192,6 +194,32 @@ class DistributedDataParallel(nn.Module):
         else:
             dist.broadcast(t, 0)
 
+    def _broadcast_bytes(self, t: torch.Tensor):
+        """The same for a uint8 tensor."""
+        if self.world_size == 1:
+            return
+        if self._comm is not None:
+            C = native()
+            self._comm.broadcast(t.data_ptr(), t.data_ptr(), t.numel(), C.DType.u8, 0,
+                                 torch.cuda.current_stream(self.device).cuda_stream)
+        elif t.is_cuda and getattr(self, "transport", None) == "peer":
+            # the peer sum is of floats: each byte as a number of its own, exact
+            wide = t.float()
+            self._broadcast(wide)
+            t.copy_(wide)
+        elif t.is_cuda:  # through the host: gloo takes CPU tensors
+            h = t.cpu()
+            dist.broadcast(h, 0)
+            t.copy_(h)
+        else:
+            dist.broadcast(t, 0)
+
+    def _broadcast_buffers(self):
+        if self.flat_buffers is not None:
+            self._broadcast(self.flat_buffers)
+        if self.flat_bytes is not None:
+            self._broadcast_bytes(self.flat_bytes)
+
     def _sync_params(self):
         with torch.no_grad():
             self._broadcast(self.flat.data)
@@ -199,8 +227,12 @@ class DistributedDataParallel(nn.Module):
                 from .. import ops
 
                 ops.invalidate_filters(self.flat.data.device)  # raw write: banked filters stale
-            if self.flat_buffers is not None:
-                self._broadcast(self.flat_buffers)
+            self._broadcast_buffers()
+            if self._counters and self.world_size > 1:
+                counts = torch.stack([c.to(torch.int64) for c in self._counters])
+                self._broadcast_bytes(counts.view(torch.uint8))
+                for c, n in zip(self._counters, counts):
+                    c.copy_(n)
 
     # ------------------------------------------------------------------ hooks
     def _make_hook(self, i: int):
@@ -227,7 +259,7 @@ class DistributedDataParallel(nn.Module):
         self.flat.attach_grads()
         if self.broadcast_buffers and self.world_size > 1 and self.module.training:
             with torch.no_grad():
-                self._broadcast(self.flat_buffers)
+                self._broadcast_buffers()
         if self._queued:
             # the previous backward raised after its first gradient hook: its finalize callback
             # never ran, so drop that step's reducer state before starting a new one

@@ -71,8 +71,7 @@ class FlatParams:
 def flatten_buffers(module: nn.Module, device: torch.device | None = None):
     """Re-home floating-point buffers (BN running stats) into one flat tensor so the DDP
     per-forward buffer broadcast (reference default broadcast_buffers=True) is ONE
-    collective.  Integer buffers (num_batches_tracked) stay separate (identical on all
-    ranks because every rank runs the same number of steps)."""
+    collective.  Integer buffers: ``flatten_integer_buffers``."""
     bufs = [(n, b) for n, b in module.named_buffers() if b is not None and b.is_floating_point()]
     if not bufs:
         return None
@@ -86,3 +85,28 @@ def flatten_buffers(module: nn.Module, device: torch.device | None = None):
         b.data = flat[off:off + n].view_as(b)
         off += _al(n)
     return flat
+
+
+def flatten_integer_buffers(module: nn.Module, device: torch.device | None = None):
+    """Re-home integer buffers (the weight of an 8-bit layer) into one flat byte tensor, broadcast
+    together with the floating-point ones: such a weight means nothing without its own scales.
+    Counters (num_batches_tracked, no dimensions) stay where they are: they are broadcast at wrap
+    time only (``integer_counters``), every rank counting the same steps from there."""
+    bufs = [b for b in module.buffers() if not b.is_floating_point() and not b.is_complex() and b.dim() > 0]
+    if not bufs:
+        return None
+    device = device or bufs[0].device
+    size = lambda b: _al(b.numel() * b.element_size() // 4 + 1) * 4  # noqa: E731 - bytes, 64-byte starts
+    flat = torch.zeros(sum(size(b) for b in bufs), dtype=torch.uint8, device=device)
+    off = 0
+    for b in bufs:
+        n = b.numel() * b.element_size()
+        home = flat[off:off + n].view(b.dtype).view(b.shape)
+        home.copy_(b)
+        b.data = home
+        off += size(b)
+    return flat
+
+
+def integer_counters(module: nn.Module) -> list[torch.Tensor]:
+    return [b for b in module.buffers() if not b.is_floating_point() and not b.is_complex() and b.dim() == 0]
