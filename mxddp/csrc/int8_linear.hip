@@ -3,7 +3,8 @@
 // quantize_rows_k: one scale per row, s = max(max|x| / 127, 2^-126), q = x / s rounded half to even.
 // The quotient is rounded as the exact one: rint(x * (1 / s)) is at most one step off, and the
 // remainder x - q s, exact in fp32 by fma (x and q s are within one s of each other and multiples of
-// the smaller one's last place), says which way.
+// the smaller one's last place), says which way.  Its double is compared with s: half of a small s
+// need not be a number of fp32.
 // int8_gemm_k: rows of q and rows of w, both contiguous in k, on v_mfma_i32_16x16x64_i8; the sum is a
 // whole number below 2^31, so it is exact in any order.
 #include <algorithm>
@@ -21,11 +22,11 @@ constexpr float kTiny = 1.17549435e-38f;  // 2^-126: its reciprocal is finite
 
 __device__ __forceinline__ int quant1(float x, float s, float inv) {
   float q = rintf(x * inv);
-  const float r = __builtin_fmaf(-q, s, x), h = 0.5f * s;
-  if (__builtin_expect(fabsf(r) >= h, 0)) {
+  const float r = __builtin_fmaf(-q, s, x), r2 = r + r;
+  if (__builtin_expect(fabsf(r2) >= s, 0)) {
     const bool odd = ((int)q & 1) != 0;
-    if (r > h || (r == h && odd)) q += 1.f;
-    else if (r < -h || (r == -h && odd)) q -= 1.f;
+    if (r2 > s || (r2 == s && odd)) q += 1.f;
+    else if (r2 < -s || (r2 == -s && odd)) q -= 1.f;
   }
   return (int)q;
 }

@@ -79,6 +79,29 @@ def test_quantize_rows_halves(dev):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+def test_quantize_rows_halves_of_small_scales(dev):
+    """The numbers next to a half at scales just above 2^-126 with an odd last place: half of such a
+    scale is no number of fp32.  A number x and a scale s are multiples of 2^-149, so a quotient
+    misses a half by nothing or by at least 2^-149 / (2 s) >= 2^-25."""
+    g = torch.Generator().manual_seed(6)
+    s = ((2**23 + torch.cat([torch.arange(1, 40, 2), torch.randint(2**22, (300,), generator=g) * 2 + 1])).double()
+         * 2.0**-149)
+    n = torch.arange(-126, 126, dtype=torch.float64) + 0.5
+    step = torch.tensor([-1.0, 0.0, 1.0], dtype=torch.float64) * 2.0**-149
+    x = ((n[None, :, None] * s[:, None, None]).float().double() + step).reshape(len(s), -1)
+    x = torch.cat([x, 127 * s[:, None]], 1).float()
+    wq, ws = oracle_quantize(x)
+    assert int((ws == s.float()).sum()) > 300  # the rows' largest magnitudes give these scales
+    q, sc = ops.quantize_rows(x.to(dev))
+    assert torch.equal(sc.cpu(), ws) and torch.equal(q.cpu(), wq)
+    # the product's own quantisation: y = q * scale * 2^126, rounded once, through a weight row of a single 1
+    w = torch.zeros(1, x.shape[1], dtype=torch.int8)
+    w[0, 7] = 1
+    y = ops.linear_int8(x[:8].to(dev), w.to(dev), torch.full((1,), 2.0**126, device=dev))
+    assert torch.equal(y.cpu()[:, 0], (wq[:8, 7].double() * ws[:8].double() * 2.0**126).float())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_quantize_rows_values(dev):
     """Rows of zeros, subnormals, the largest numbers, and rows that are not finite."""
     big = torch.finfo(torch.float32).max
