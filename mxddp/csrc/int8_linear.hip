@@ -194,12 +194,18 @@ struct Four {
   }
   template <class T>
   __device__ __forceinline__ void put(const GemmArgs& a, int64_t m, int n, i32x4 acc, float xs) const {
+    float f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = __builtin_fmaf((float)acc[e] * xs, ws[e], b[e]);
+    // A token's scale with which the first product could leave fp32 at either end (|acc| < 2^31), though
+    // the channel's scale brings it back: in 64 bits.
+    if (__builtin_expect(!(fabsf(xs) >= kTiny && fabsf(xs) < 0x1p96f), 0)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = (float)((double)acc[e] * xs * ws[e] + b[e]);
+    }
     typename T::store_t v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float f = (float)acc[e] * xs * ws[e] + b[e];
-      v[e] = T::store(a.relu && f < 0.f ? 0.f : f);  // a NaN stays one
-    }
+    for (int e = 0; e < 4; ++e) v[e] = T::store(a.relu && f[e] < 0.f ? 0.f : f[e]);  // a NaN stays one
     typename T::store_t* o = static_cast<typename T::store_t*>(a.y) + m * a.N + n;
     if (n + 3 < a.N) {
       __builtin_memcpy(o, v, sizeof(v));

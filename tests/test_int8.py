@@ -332,6 +332,30 @@ def test_linear_int8_values(dev):
     assert (y == 0).all()
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("M", [1, 24, 70, 600])
+def test_linear_int8_far_scales(dev, M):
+    """Tokens of very large or very small values beside channel scales that bring the result back:
+    no step of the epilogue leaves fp32's range where the result does not."""
+    N, K = 130, 64
+    x, w, _, b = make(M, N, K, torch.float32, M)
+    x = x / x.abs().amax(1, keepdim=True)
+    for top, scale, bias in ((1e37, 1e-8, 1e30), (3e38, 1e-30, 1.0), (1.0, 1e30, 1e30), (1e38, 1e-5, 1e38)):
+        xt, ws, bt = x * top, (torch.rand(N, generator=torch.Generator().manual_seed(1)) + 0.5) * scale, b * bias
+        q, s = oracle_quantize(xt)
+        assert bool(torch.isfinite(oracle_linear(q, s, w, ws, bt, False)[0].float()).all())
+        check_linear(ops.linear_int8(xt.to(dev), w.to(dev), ws.to(dev), bt.to(dev)), q, s, w, ws, bt, False)
+        check_linear(ops.linear_int8(xt.to(dev), w.to(dev), ws.to(dev), relu=True), q, s, w, ws, None, True)
+    # scales that are given: subnormal ones, the largest, zero and a negative one
+    q = torch.randint(-127, 128, (M, K), generator=torch.Generator().manual_seed(2), dtype=torch.int8)
+    for xs, scale in ((3e-42, 1e30), (3e38, 1e-10), (0.0, 1e30), (-3e37, 1e-10)):
+        s = torch.full((M,), xs)
+        s[::2] = 0.25  # tokens of ordinary scales beside them
+        ws = torch.full((N,), scale)
+        y = ops.linear_int8(q.to(dev), w.to(dev), ws.to(dev), b.to(dev), x_scale=s.to(dev))
+        check_linear(y, q, s, w, ws, b, False)
+
+
 def test_refusals():
     x, w, ws, b = make(4, 6, 8, torch.float32)
     for bad, err in [
