@@ -46,6 +46,11 @@ def quantize_rows(x: torch.Tensor):
     return q, scale
 
 
+def _row_stride(t):
+    """Of a [rows, K] tensor; a single row has none that matters, whatever it was cut from: whole pieces."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
 def _room(w, K):
     """Bytes that may be read of each of w's rows: whole 16-byte pieces where its memory goes on."""
     pieces = (K + 15) // 16 * 16
@@ -103,18 +108,18 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     M = x2.shape[0]
     if M > MAX_ROWS:
         raise ValueError(f"linear_int8: {M} rows, at most {MAX_ROWS}")
-    if (weight.stride(1) != 1 and K > 1) or weight.stride(0) > _MAX_LD:
+    if (weight.stride(1) != 1 and K > 1) or _row_stride(weight) > _MAX_LD:
         weight = weight.contiguous()
     weight_scale = weight_scale.contiguous()
     bias = None if bias is None else bias.contiguous()
     y = torch.empty((*x.shape[:-1], N), device=x.device, dtype=out_dtype)
     C, xt, yt = native(), DTYPES.get(x2.dtype, -1), DTYPES[out_dtype]
-    wargs = (weight.data_ptr(), weight.stride(0), _room(weight, K), weight_scale.data_ptr(), _p(bias), y.data_ptr(), yt,
+    wargs = (weight.data_ptr(), _row_stride(weight), _room(weight, K), weight_scale.data_ptr(), _p(bias), y.data_ptr(), yt,
              M, N, K, bool(relu))
     with on_device(x2):
         if given:
-            x2 = x2 if x2.stride(0) <= _MAX_LD else x2.contiguous()
-            C.linear_int8(x2.data_ptr(), x2.stride(0), K, x_scale.contiguous().data_ptr(), *wargs, stream(x2))
+            x2 = x2 if _row_stride(x2) <= _MAX_LD else x2.contiguous()
+            C.linear_int8(x2.data_ptr(), _row_stride(x2), K, x_scale.contiguous().data_ptr(), *wargs, stream(x2))
         else:
             n = C.linear_int8_scratch(xt, yt, M, K)
             scratch = torch.empty((n,), device=x2.device, dtype=torch.int8) if n else None

@@ -356,6 +356,32 @@ def test_linear_int8_far_scales(dev, M):
         check_linear(y, q, s, w, ws, b, False)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("K", [1, 100, 4096])
+def test_linear_int8_one_row_of_a_wide_tensor(dev, K):
+    """A single row keeps the stride of the tensor it was cut from, however large: the last token of a
+    sequence, a weight of one output channel, both."""
+    T = (2**22 + K) // K + 1  # rows of T K > 2^22 elements
+    g = torch.Generator().manual_seed(K)
+    q = torch.randint(-127, 128, (1, T, K), generator=g, dtype=torch.int8)
+    s = torch.rand(1, T, generator=g)
+    w = torch.randint(-127, 128, (70, K), generator=g, dtype=torch.int8)
+    ws = torch.rand(70, generator=g) * 1e-3
+    qd, sd, wd, wsd = (t.to(dev) for t in (q, s, w, ws))
+    y = ops.linear_int8(qd[:, -1], wd, wsd, x_scale=sd[:, -1])
+    check_linear(y, q[:, -1], s[:, -1], w, ws, None, False)
+    one = qd.reshape(1, T * K)[:, 3 * K:4 * K]  # the same for a weight
+    y = ops.linear_int8(wd, one, wsd[:1], x_scale=wsd)
+    check_linear(y, w, ws, one.cpu(), ws[:1], None, False)
+    y = ops.linear_int8(qd[:, -2], one, wsd[:1], x_scale=sd[:, -2])
+    check_linear(y, q[:, -2], s[:, -2], one.cpu(), ws[:1], None, False)
+    x = qd.float()[:, -1]
+    xq, xs = oracle_quantize(x)
+    check_linear(ops.linear_int8(x, one, wsd[:1]), xq, xs, one.cpu(), ws[:1], None, False)
+    gq, gs = ops.quantize_rows(x)
+    assert torch.equal(gq.cpu(), xq) and torch.equal(gs.cpu(), xs)
+
+
 def test_refusals():
     x, w, ws, b = make(4, 6, 8, torch.float32)
     for bad, err in [
