@@ -620,7 +620,7 @@ void launch_skinny(GemmArgs a, hipStream_t st, const void* x = nullptr, int64_t 
 
 void quantize_rows(const void* x, int xtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K,
                    hipStream_t st) {
-  MX_CHECK(rows >= 0 && rows <= kMaxRows && K >= 1 && ldq >= K, "quantize_rows: bad sizes");
+  MX_CHECK(rows >= 0 && rows <= kMaxRows && K >= 1 && K <= kMaxLength && ldq >= K, "quantize_rows: bad sizes");
   if (rows == 0) return;
   // one wave where a row fits its registers: no barrier
   MX_BY_TYPE(xtype, T, {
@@ -636,7 +636,8 @@ void quantize_rows(const void* x, int xtype, int64_t ldx, int8_t* q, int64_t ldq
 void linear_int8(const int8_t* q, int64_t ldq, int q_room, const float* xs, const int8_t* w, int64_t ldw, int w_room,
                  const float* ws, const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu,
                  hipStream_t st) {
-  MX_CHECK(M >= 0 && M <= kMaxRows && N >= 1 && K >= 1 && K <= kInt8MaxK, "linear_int8: bad sizes");
+  MX_CHECK(M >= 0 && M <= kMaxRows && N >= 1 && N <= kMaxLength && K >= 1 && K <= kInt8MaxK,
+           "linear_int8: bad sizes");
   MX_CHECK(ldq >= 0 && ldq <= kInt8MaxLd && ldw >= 0 && ldw <= kInt8MaxLd, "linear_int8: row stride too large");
   if (M == 0) return;
   GemmArgs a{q, w, xs, ws, bias, y, ldq, ldw, M, N, K, relu ? 1 : 0, 0, 0};
@@ -697,7 +698,8 @@ int64_t linear_int8_scratch(int xtype, int ytype, int64_t M, int K) {
 void linear_int8_float(const void* x, int xtype, int64_t ldx, const int8_t* w, int64_t ldw, int w_room, const float* ws,
                        const float* bias, void* y, int ytype, int64_t M, int N, int K, bool relu, void* scratch,
                        hipStream_t st) {
-  MX_CHECK(M >= 0 && M <= kMaxRows && N >= 1 && K >= 1 && K <= kInt8MaxK && ldw >= 0 && ldw <= kInt8MaxLd,
+  MX_CHECK(M >= 0 && M <= kMaxRows && N >= 1 && N <= kMaxLength && K >= 1 && K <= kInt8MaxK && ldw >= 0 &&
+               ldw <= kInt8MaxLd,
            "linear_int8: bad sizes");
   if (M == 0) return;
   if (quantises(xtype, ytype, M, K)) {

@@ -293,6 +293,8 @@ void augment_crop_flip_norm(const float* x, float* y, int N, int C, int H, int W
                             hipStream_t st);
 // most rows (blocks of up to 512 threads) that one launch of the following takes: 2^32 threads
 constexpr int64_t kMaxRows = (1 << 23) - 1;
+// longest row, and most channels of a layer: with a tile more it is still an int
+constexpr int kMaxLength = 1 << 30;
 
 // ---- linear layers in 8-bit integers (int8_linear.hip); element types: lowp.h DType ----
 // |q w| <= 2^14, so up to this many products sum to less than 2^31

@@ -13,6 +13,7 @@ from . import _native, _p
 from .lowp import DTYPES, MAX_ROWS, check_device, check_float, on_device, rows_of, stream
 
 MAX_K = 2**17 - 1  # products of 2^14 each whose sum stays below 2^31
+MAX_LENGTH = 2**30   # csrc/ops.h kMaxLength: of a row that is quantised, and channels of a layer
 _TINY = 2.0**-126
 _MAX_LD = 2**22      # csrc/ops.h kInt8MaxLd
 
@@ -22,10 +23,11 @@ def quantize_rows(x: torch.Tensor):
 
     ``scale = max|x| / 127`` (at least 2^-126) and ``q = x / scale`` rounded half to even, exactly.
     A row with an infinity or a NaN has a NaN scale and q = 0.  ``x``: [..., K], float32, bfloat16
-    or float16, at most 8388607 rows.  Weights [out, in] give the per-channel scales that ``linear_int8`` takes."""
+    or float16, at most 8388607 rows, K at most 2^30.  Weights [out, in] give the per-channel scales that
+    ``linear_int8`` takes."""
     check_float(x, "quantize_rows: x")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"quantize_rows: x must be [..., K] with K >= 1, got {tuple(x.shape)}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_LENGTH:
+        raise ValueError(f"quantize_rows: x must be [..., K] with 1 <= K <= 2^30, got {tuple(x.shape)}")
     x = x.detach()
     if not _native(x):
         xd = x.double()
@@ -68,7 +70,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     ``bias``: float32 [N].  ``x``: [..., K] in float32, bfloat16 or float16, or int8 with its
     ``x_scale`` [...] (``quantize_rows``: one quantised input for several layers).  The result has
     ``out_dtype`` (default: x's type, float32 for an int8 x).  K is at most 131071, and x has at most
-    8388607 rows.  No gradient: an input that requires one is refused while autograd records.
+    8388607 rows.  N is at most 2^30; on the GPU a layer of more than 134217712 channels (2^27 - 16) may
+    be refused.  No gradient: an input that requires one is refused while autograd records.
 
     Rows of whole 16-byte pieces (K a multiple of 16, or a weight with padded rows as ``Int8Linear``
     keeps it) take the faster way into the large tiles."""
@@ -77,8 +80,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     N, K = weight.shape
     if weight.dtype != torch.int8:
         raise TypeError(f"linear_int8: weight must be int8, got {weight.dtype}")
-    if not 1 <= K <= MAX_K or N < 1:
-        raise ValueError(f"linear_int8: weight {tuple(weight.shape)}: 1 <= K <= {MAX_K} and N >= 1")
+    if not 1 <= K <= MAX_K or not 1 <= N <= MAX_LENGTH:
+        raise ValueError(f"linear_int8: weight {tuple(weight.shape)}: 1 <= K <= {MAX_K} and 1 <= N <= 2^30")
     given = x.dtype == torch.int8
     if given:
         if x_scale is None or x_scale.dtype != torch.float32 or x_scale.shape != x.shape[:-1]:

@@ -413,6 +413,27 @@ def test_refusals():
         ops.linear_int8(x.clone().requires_grad_(), w, ws)
 
 
+def test_refusals_of_lengths():
+    """Rows and layers whose ends the kernels' 32-bit places do not reach, on either device; the native
+    entries refuse them before anything is launched."""
+    from mxddp import native
+
+    C = native()
+    one = torch.zeros(1, 1, dtype=torch.bfloat16)
+    for n in (2**30 + 1, 2**31 - 1, 2**31, 2**32 + 5):
+        with pytest.raises(ValueError, match=r"2\^30"):
+            ops.quantize_rows(one.expand(1, n))
+        with pytest.raises(ValueError, match=r"2\^30"):
+            ops.linear_int8(one, one.to(torch.int8).expand(n, 1), torch.ones(1).expand(n))
+    for n in (2**30 + 1, 2**31 - 1):
+        with pytest.raises(RuntimeError, match="bad sizes"):
+            C.quantize_rows(0, 1, n, 0, n, 0, 1, n, 0)
+        with pytest.raises(RuntimeError, match="bad sizes"):
+            C.linear_int8(0, 16, 16, 0, 0, 16, 16, 0, 0, 0, 0, 1, n, 16, False, 0)
+        with pytest.raises(RuntimeError, match="bad sizes"):
+            C.linear_int8_float(0, 1, 16, 0, 16, 16, 0, 0, 0, 1, 1, n, 16, False, 0, 0)
+
+
 @pytest.mark.gpu
 def test_refusals_native(cuda):
     """The native entries refuse sizes that their kernels do not take."""
