@@ -35,7 +35,9 @@ class Linear(nn.Linear):
 class Int8Linear(nn.Module):
     """A trained ``Linear`` for answering in 8-bit integers (``ops.linear_int8``): int8 weight with a
     scale per output channel, inputs quantised per row on the fly, the ReLU in the epilogue.  No
-    parameters and no gradient; ``weight`` rows are padded with zeros to whole 16-byte pieces."""
+    parameters and no gradient; ``weight`` rows are padded with zeros to whole 16-byte pieces.  A cast
+    of the module (``half()``, ``to(torch.bfloat16)``) leaves its buffers' types and values as they
+    are: the layer takes and answers in the type of its input."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, fuse_relu: bool = False):
         super().__init__()
@@ -56,6 +58,15 @@ class Int8Linear(nn.Module):
         if layer.bias is not None:
             new.bias.copy_(layer.bias)
         return new
+
+    def _apply(self, fn, recurse=True):
+        before = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, old in before.items():
+            new = self._buffers[name]
+            if old is not None and new.dtype != old.dtype:
+                self._buffers[name] = old.to(new.device)
+        return self
 
     def forward(self, x):
         return ops.linear_int8(x, self.weight[:, :self.in_features], self.weight_scale, self.bias, relu=self.fuse_relu)

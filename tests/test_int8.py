@@ -502,3 +502,35 @@ def test_int8_linear_layer(dev, bias, relu, K):
     with torch.no_grad():
         assert torch.equal(other(x.to(dev)), y)
     assert sum(p.numel() for p in lay.parameters()) == 0
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("cast", ["half", "bfloat16", "double", "to", "type", "to_device"])
+def test_int8_linear_layer_casts(dev, cast):
+    """A whole model cast to another type, its 8-bit layers in it: they keep their bits and take inputs of
+    the type; casting back and forth changes nothing; a move to a device goes through."""
+    torch.manual_seed(1)
+    lin = Linear(40, 30, fuse_relu=True)
+    model = torch.nn.Sequential(Int8Linear.from_linear(lin), torch.nn.Identity(), Int8Linear.from_linear(Linear(30, 7)))
+    want = {k: v.clone() for k, v in model.state_dict().items()}
+    to = {"half": lambda m: m.half(), "bfloat16": lambda m: m.bfloat16(), "double": lambda m: m.double(),
+          "to": lambda m: m.to(torch.float16), "type": lambda m: m.type(torch.bfloat16),
+          "to_device": lambda m: m.to(dev, torch.bfloat16)}[cast]
+    assert to(model) is model
+    model.to(dev)
+    for _ in range(2):
+        got = model.state_dict()
+        assert list(got) == list(want)
+        for k, v in got.items():
+            assert v.device.type == dev and v.dtype == want[k].dtype and torch.equal(v.cpu(), want[k]), k
+        model.half().float()
+    for dtype in TYPES:
+        x = torch.randn(6, 40, generator=torch.Generator().manual_seed(2)).to(dtype)
+        y = model[0](x.to(dev))
+        assert y.dtype == dtype
+        q, s = oracle_quantize(x)
+        check_linear(y, q, s, want["0.weight"][:, :40], want["0.weight_scale"], want["0.bias"], True)
+        assert model(x.to(dev)).dtype == dtype
+    assert Int8Linear(5, 3, bias=False).half().bias is None
+    empty = Int8Linear(5, 3).to("meta").half().to_empty(device=dev)
+    assert empty.weight_scale.dtype == torch.float32 and empty.weight.device.type == dev
