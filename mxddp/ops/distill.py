@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import native
 from . import _native, _p
-from .lowp import DTYPES, MAX_ROWS, check_device, check_float, on_device, rows_of, stream
+from .lowp import DTYPES, MAX_ROWS, check_device, check_float, has_derivative, on_device, rows_of, stream
 
 MAX_TOP = 256       # csrc/ops.h kTopMax
 MAX_CLASSES = 2**30
@@ -40,7 +40,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     ``logits``: [..., V] float32, bfloat16 or float16, at most 8388607 rows and 2^30 classes;
     1 <= k <= min(V, 256).  A NaN counts as the
     largest value.  ``lse`` is taken at ``temperature`` over all classes (infinite or NaN where the
-    largest logit is).  The results carry no gradient."""
+    largest logit is).  The results carry no derivative, as those of ``detach``."""
     check_float(logits, "top_logits: logits")
     if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_CLASSES:
         raise ValueError(f"top_logits: logits must be [..., V] with 1 <= V <= 2^30, got {tuple(logits.shape)}")
@@ -166,7 +166,7 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torc
     as -100) is left out: loss 0, gradient 0, not counted.  Without targets the rows with no used
     entry are left out.  ``reduction``: "mean" over the counted rows (0 if there are none), "sum", or
     "none" (each row's loss, [...]).  The loss is float32.  Only ``logits`` get a gradient, once
-    differentiable.
+    differentiable; on the GPU a forward-mode tangent is refused.
 
     Both directions may be captured into a graph.  As for every operator, no loss of an earlier eager
     step may then still hold its autograd graph: torch would draw the stream on which that step met
@@ -193,7 +193,7 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torc
                          f"{tuple(top_lse.shape)}")
     for t, name in ((top_values, "top_values"), (top_index, "top_index"), (target, "target"), (top_lse, "top_lse")):
         check_device(t, logits, name)
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
+        if has_derivative(t):
             raise ValueError(f"distill_loss: {name} gets no gradient; detach it")
     temperature, hard = _check_temperature(temperature), float(hard_weight)
     if not 0 <= hard <= 1:

@@ -10,7 +10,7 @@ import torch
 
 from .. import native
 from . import _native, _p
-from .lowp import DTYPES, MAX_ROWS, check_device, check_float, on_device, rows_of, stream
+from .lowp import DTYPES, MAX_ROWS, check_device, check_float, has_derivative, on_device, rows_of, stream
 
 MAX_K = 2**17 - 1  # products of 2^14 each whose sum stays below 2^31
 MAX_LENGTH = 2**30   # csrc/ops.h kMaxLength: of a row that is quantised, and channels of a layer
@@ -24,7 +24,7 @@ def quantize_rows(x: torch.Tensor):
     ``scale = max|x| / 127`` (at least 2^-126) and ``q = x / scale`` rounded half to even, exactly.
     A row with an infinity or a NaN has a NaN scale and q = 0.  ``x``: [..., K], float32, bfloat16
     or float16, at most 8388607 rows, K at most 2^30.  Weights [out, in] give the per-channel scales that
-    ``linear_int8`` takes."""
+    ``linear_int8`` takes.  The results carry no derivative, as those of ``detach``."""
     check_float(x, "quantize_rows: x")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_LENGTH:
         raise ValueError(f"quantize_rows: x must be [..., K] with 1 <= K <= 2^30, got {tuple(x.shape)}")
@@ -71,7 +71,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     ``x_scale`` [...] (``quantize_rows``: one quantised input for several layers).  The result has
     ``out_dtype`` (default: x's type, float32 for an int8 x).  K is at most 131071, and x has at most
     8388607 rows.  N is at most 2^30; on the GPU a layer of more than 134217712 channels (2^27 - 16) may
-    be refused.  No gradient: an input that requires one is refused while autograd records.
+    be refused.  No gradient: an input that requires one is refused while autograd records, and one with
+    a forward-mode tangent always.
 
     Rows of whole 16-byte pieces (K a multiple of 16, or a weight with padded rows as ``Int8Linear``
     keeps it) take the faster way into the large tiles."""
@@ -90,8 +91,9 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         check_float(x, "linear_int8: x")
         if x_scale is not None:
             raise ValueError("linear_int8: x_scale goes with an int8 x")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight_scale, bias, x_scale)):
-        raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad() or detach its inputs")
+    if has_derivative(x, weight_scale, bias, x_scale):
+        raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad() or detach its inputs "
+                           "(detach those with a forward-mode tangent)")
     out_dtype = out_dtype or (torch.float32 if given else x.dtype)
     if out_dtype not in DTYPES:
         raise TypeError(f"linear_int8: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")

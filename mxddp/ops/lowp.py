@@ -4,6 +4,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # csrc/lowp.h DType
 MAX_ROWS = 2**23 - 1  # csrc/ops.h kMaxRows
@@ -17,6 +18,15 @@ def check_float(t: torch.Tensor, name: str, cpu_double: bool = False) -> None:
 def check_device(t: torch.Tensor | None, x: torch.Tensor, name: str) -> None:
     if t is not None and t.device != x.device:
         raise ValueError(f"{name} is on {t.device}, the input on {x.device}")
+
+
+def has_derivative(*tensors: torch.Tensor | None) -> bool:
+    """Whether autograd would carry a derivative through any of these: backward while it records, or a
+    forward-mode tangent (which torch.no_grad does not turn off)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                  for t in tensors)
 
 
 def rows_of(t: torch.Tensor) -> torch.Tensor:

@@ -12,6 +12,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from mxddp import ops
 from mxddp.models.layers import Int8Linear, Linear
@@ -484,6 +485,30 @@ def test_refusals():
     ]:
         with pytest.raises(err):
             bad()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_forward_mode_derivatives(dev):
+    """The teacher's side with a tangent is refused, top_logits' results carry none; the student's gives
+    the right one (CPU path) or is refused."""
+    z, tv, ti, y, lse = (t.to(dev) for t in make(4, 30, 3, torch.float32))
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for bad in (lambda: ops.distill_loss(z, dual(tv), ti), lambda: ops.distill_loss(z, tv, ti, top_lse=dual(lse))):
+            with pytest.raises(ValueError, match="detach"):
+                bad()
+            with torch.no_grad(), pytest.raises(ValueError, match="detach"):
+                bad()
+        got = ops.top_logits(dual(z), 3)
+        assert all(forward_ad.unpack_dual(t).tangent is None for t in (got.values, got.lse))
+        d = torch.randn(4, 30, generator=torch.Generator().manual_seed(1)).to(dev)
+        if dev == "cuda":
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                ops.distill_loss(forward_ad.make_dual(z, d), tv, ti)
+        else:
+            slope = forward_ad.unpack_dual(ops.distill_loss(forward_ad.make_dual(z.double(), d.double()), tv, ti)).tangent
+            _, _, grad, _, _ = oracle(z, tv, ti, None, None, 1.0, 0.0)
+            assert abs(slope - (grad * d).sum() / 4) < 1e-12
 
 
 @pytest.mark.parametrize("t", [0.0, -1.0, 1e-40, 1e-31, 1e31, float("inf"), float("nan")])

@@ -9,6 +9,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from mxddp import ops
 from mxddp.models.layers import Int8Linear, Linear
@@ -534,3 +535,25 @@ def test_int8_linear_layer_casts(dev, cast):
     assert Int8Linear(5, 3, bias=False).half().bias is None
     empty = Int8Linear(5, 3).to("meta").half().to_empty(device=dev)
     assert empty.weight_scale.dtype == torch.float32 and empty.weight.device.type == dev
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_forward_mode_derivatives(dev):
+    """linear_int8 refuses every input with a tangent (under no_grad too, which leaves forward mode on);
+    quantize_rows' results carry none."""
+    x, w, ws, b = (t.to(dev) for t in make(4, 6, 8, torch.float32))
+    q, s = ops.quantize_rows(x)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for bad in (lambda: ops.linear_int8(dual(x), w, ws), lambda: ops.linear_int8(x, w, dual(ws)),
+                    lambda: ops.linear_int8(x, w, ws, dual(b)), lambda: ops.linear_int8(q, w, ws, x_scale=dual(s))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                bad()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                bad()
+        gq, gs = ops.quantize_rows(dual(x))
+        assert forward_ad.unpack_dual(gs).tangent is None and torch.equal(gq, q) and torch.equal(gs, s)
+        y = ops.linear_int8(x, w, ws, b)
+    assert torch.equal(y, ops.linear_int8(x, w, ws, b))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda v: ops.linear_int8(v, w, ws), (x,), (x,))
