@@ -733,14 +733,15 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, co
                     : all_s > 0 ? 0.0 : __builtin_nan("");  // a row of -inf has no distribution
   const float ref = has_out ? out.m : top;
   const double h = a.hard, z1 = two ? all_s1 : all_s;
-  double loss = (1 - h) * a.temperature * a.temperature * kd;
+  // a weight of 0 takes the term out, whatever the teacher says (KD is infinite where a named class is masked)
+  const double w = (1 - h) * a.temperature;
+  double loss = w == 0 ? 0.0 : w * a.temperature * kd;
   if (h > 0) loss += h * (log(z1) - ((double)T::load(z[r.y]) - top));
   loss_rows[row] = (float)loss;
-  const double w = (1 - h) * a.temperature;
   st[0] = ref;
-  st[1] = (float)(w * co + (h > 0 && !two ? h * exp((double)ref - top) / z1 : 0.0));
+  st[1] = (float)((w == 0 ? 0.0 : w * co) + (h > 0 && !two ? h * exp((double)ref - top) / z1 : 0.0));
   st[2] = top;
-  st[3] = r.any ? (float)(w * mass / all_s) : 0.f;
+  st[3] = r.any && w != 0 ? (float)(w * mass / all_s) : 0.f;
   st[4] = h > 0 ? (float)(h / z1) : 0.f;
   st[5] = 1.f;
   *reinterpret_cast<double*>(st + 6) = norm;  // all its bits: with a small T it is large, and u near it
@@ -894,7 +895,7 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
   load_entry(a, row, inv_t, &cls, &u);
   cls_s[tid] = cls;
   const double norm = *reinterpret_cast<const double*>(st + 6);
-  p_s[tid] = cls >= 0 ? (float)((1 - a.hard) * a.temperature * exp(u - norm)) : 0.f;
+  p_s[tid] = cls >= 0 && a.hard < 1 ? (float)((1 - a.hard) * a.temperature * exp(u - norm)) : 0.f;
   const int64_t y = a.hard > 0 ? load_int(a.target, row, a.target64) : -1;
   __syncthreads();  // also orders the stores above before the ones below
   if (cls >= begin && cls < end) {

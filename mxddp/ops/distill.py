@@ -108,13 +108,9 @@ class _DistillLoss(torch.autograd.Function):
         return dz, None, None, None, None, None, None, None
 
 
-def _distill_rows(z, tv, ti, target, tlse, temperature, hard):
-    """Each row's loss in plain torch (the CPU path), in 64 bits, and which rows count."""
+def _distill_kd(z, tv, ti, tlse, temperature, used, counted):
+    """Each row's KL(p || q), in 64 bits."""
     V = z.shape[1]
-    used = (ti >= 0) & (ti < V) & (tv != -math.inf)
-    counted = used.any(1) if target is None else (target >= 0) & (target < V)
-    z = torch.where(counted[:, None], z.double(), 0.0)  # what a left-out row holds stays out
-    used = used & counted[:, None]
     at = torch.where(used, ti, 0).long()
     zt = z / temperature
     total = torch.logsumexp(zt, 1)
@@ -136,8 +132,19 @@ def _distill_rows(z, tv, ti, target, tlse, temperature, hard):
         outside = torch.logsumexp(torch.where(named & has[:, None], -math.inf, zt), 1)
         safe = torch.where(has, rest, 1.0)
         kd = kd + torch.where(has, safe * (safe.log() - (outside - total)), 0.0)
-    kd = torch.where(used.any(1), kd, 0.0) if tlse is None else kd
-    loss = (1 - hard) * temperature * temperature * kd
+    return torch.where(used.any(1), kd, 0.0) if tlse is None else kd
+
+
+def _distill_rows(z, tv, ti, target, tlse, temperature, hard):
+    """Each row's loss in plain torch (the CPU path), in 64 bits, and which rows count."""
+    V = z.shape[1]
+    used = (ti >= 0) & (ti < V) & (tv != -math.inf)
+    counted = used.any(1) if target is None else (target >= 0) & (target < V)
+    z = torch.where(counted[:, None], z.double(), 0.0)  # what a left-out row holds stays out
+    used = used & counted[:, None]
+    loss = torch.zeros_like(z[:, 0])
+    if hard < 1:  # a weight of 0 takes the term out, whatever the teacher says
+        loss = (1 - hard) * temperature * temperature * _distill_kd(z, tv, ti, tlse, temperature, used, counted)
     if hard > 0:
         y = torch.where(counted, target, 0).long()[:, None]
         loss = loss + hard * (torch.logsumexp(z, 1) - z.gather(1, y)[:, 0])
@@ -150,6 +157,8 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torc
     """Distillation from a teacher's top logits; with p the teacher's and q = softmax(logits / T)
 
         loss = (1 - hard_weight) T^2 KL(p || q) + hard_weight cross_entropy(logits, target)
+
+    (a term whose weight is 0 is left out, so with a weight of 1 the teacher's values are not looked at).
 
     ``logits``: [..., V], the student's, float32, bfloat16 or float16, at most 8388607 rows and 2^30
     classes.  ``top_values`` [..., k] (one

@@ -328,6 +328,32 @@ def test_distill_loss_far_values(dev):
         check_distill(dev, z, tv, ti, y if h else None, None, T, h)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("T", [1.0, 2.0])
+def test_distill_loss_labels_alone(dev, dtype, tail, T):
+    """hard_weight = 1 is the labels' cross-entropy: named classes that the student masks, teacher's
+    values that are infinite or NaN and rows without any change nothing."""
+    N, V, k = 6, 300, 5
+    z, tv, ti, y, lse = make(N, V, k, dtype, 21, T)
+    y = torch.where(y == ti[:, 0], (y + 1) % V, y)
+    y[1] = ti[1, 1]
+    z[0, ti[0, 0].long()] = -INF
+    z[1, ti[1, 0].long()] = -INF
+    tv[2, 1], tv[3, 0], ti[4] = INF, float("nan"), -1
+    lse[5] = -1e30  # a normaliser that does not belong to the values: p overflows
+    check_distill(dev, z[4:5], tv[4:5], ti[4:5], y[4:5], lse[4:5] if tail else None, T, 1.0)
+    rows, counted, grad, tl, tg = oracle(z, tv, torch.full_like(ti, -1), y, None, T, 1.0)
+    leaf = z.to(dev).requires_grad_()
+    loss = ops.distill_loss(leaf, tv.to(dev), ti.to(dev), y.to(dev), lse.to(dev) if tail else None, T, 1.0, "none")
+    g, = torch.autograd.grad(loss.sum(), leaf)
+    assert bool(((loss.detach().cpu().double() - rows).abs() <= tl).all())
+    fi = torch.finfo(dtype)
+    tol = tg + fi.eps / 2 * (grad.abs() + tg) + fi.smallest_normal * fi.eps
+    assert bool(((g.cpu().double() - grad).abs() <= tol).all())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [65537, 140001])
