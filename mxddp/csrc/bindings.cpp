@@ -293,7 +293,7 @@ PYBIND11_MODULE(_C, m) {
     distill_fwd(DistillArgs{P<const void>(z), P<const void>(tv), P<const void>(ti), P<const void>(target),
                             P<const float>(tlse), P<float>(stats), ldz, rows, V, k, type, tv_type, ti64, target64,
                             temperature, hard},
-                P<float>(loss_rows), P<float>(loss), mean, P<float>(scratch), S(st));
+                P<float>(loss_rows), P<float>(loss), mean, P<void>(scratch), S(st));
   });
   m.def("distill_scratch", &distill_scratch);
   m.def("distill_bwd", [](uintptr_t z, uintptr_t tv, uintptr_t ti, uintptr_t target, uintptr_t tlse, uintptr_t stats,

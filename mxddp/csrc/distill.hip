@@ -103,7 +103,7 @@ struct TileSum {
     return s > 0.f ? s * exp2_raw(-__builtin_fmaf(m, c, -R)) : s;
   }
 };
-__device__ __forceinline__ bool unsettled(float m, float s, float c) { return !(s > 0.f) || !(fabsf(m * c) < INFINITY); }
+__device__ __forceinline__ bool unsettled(float m, double s, float c) { return !(s > 0.f) || !(fabsf(m * c) < INFINITY); }
 
 // over a block of TB threads; every thread gets the result
 template <int TB>
@@ -504,27 +504,77 @@ __device__ __forceinline__ int64_t load_int(const void* p, int64_t i, int is64) 
   return is64 ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
 }
 
-__device__ __forceinline__ double block_sum_d(double v, double* red) {
+// sums over a block of each of v[0 .. NV - 1]; every thread gets them
+template <int NV>
+__device__ __forceinline__ void block_sums(double* v, double* red) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  for (int o = 32; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] += __shfl_xor(v[i], o, 64);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) red[NV * (threadIdx.x >> 6) + i] = v[i];
   __syncthreads();
-  double t = 0;
-  for (int w = 0; w < kT / 64; ++w) t += red[w];
-  return t;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    v[i] = 0;
+    for (int w = 0; w < kT / 64; ++w) v[i] += red[NV * w + i];
+  }
+}
+// maxima over a block, NaN left aside
+__device__ __forceinline__ float2 block_max2(float2 v, double* red) {
+  float2* r = reinterpret_cast<float2*>(red);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    v.x = fmaxf(v.x, __shfl_xor(v.x, o, 64));
+    v.y = fmaxf(v.y, __shfl_xor(v.y, o, 64));
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+  __syncthreads();
+  for (int w = 0; w < kT / 64; ++w) {
+    v.x = fmaxf(v.x, r[w].x);
+    v.y = fmaxf(v.y, r[w].y);
+  }
+  return v;
 }
 
-// what a row's named entries are: class (or -1) and t_j / T; k <= kT, one entry a thread
-__device__ __forceinline__ void load_entry(const DistillArgs& a, int64_t row, double inv_t, int* cls, double* u) {
+// exp(x) - 1 for x <= 0 within a few parts in 2^53 of its size: x = k log 2 + f with |f| <= 0.35, and
+// the power series of exp(f) - 1, whose first term left out is below 2^-55 of f
+__device__ __forceinline__ double expm1_neg(double x) {
+  x = x < -800.0 ? -800.0 : x;  // -1 from there on; a NaN stays one
+  const double k = rint(x * kLog2e);
+  const double f = __builtin_fma(-k, 2.3190468138462996e-17, __builtin_fma(-k, 0.6931471805599453, x));
+  double r = 1.0 / 6227020800.0;
+  constexpr double c[12] = {1.0,         1.0 / 2,     1.0 / 6,      1.0 / 24,      1.0 / 120,      1.0 / 720,
+                            1.0 / 5040,  1.0 / 40320, 1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600};
+#pragma unroll
+  for (int i = 11; i >= 0; --i) r = __builtin_fma(r, f, c[i]);
+  const double s = ldexp(1.0, (int)k);
+  return __builtin_fma(s, r * f, s - 1.0);
+}
+// x e^x - e^x + 1 = sum x^n (n - 1) / n!, for |x| <= 1/4: the first term left out is below 2^-54 of the sum
+__device__ __forceinline__ double gain_near(double x) {
+  double r = 0;
+  constexpr double c[13] = {1.0 / 2,           2.0 / 6,           3.0 / 24,          4.0 / 120,         5.0 / 720,
+                            6.0 / 5040,        7.0 / 40320,       8.0 / 362880,      9.0 / 3628800,     10.0 / 39916800,
+                            11.0 / 479001600,  12.0 / 6227020800.0, 13.0 / 87178291200.0};
+#pragma unroll
+  for (int i = 12; i >= 0; --i) r = __builtin_fma(r, x, c[i]);
+  return r * x * x;
+}
+
+// what a row's named entries are: class (or -1) and its teacher logit; k <= kT, one entry a thread
+__device__ __forceinline__ void load_entry(const DistillArgs& a, int64_t row, int* cls, float* t) {
   *cls = -1;
-  *u = 0;
+  *t = 0;
   if ((int)threadIdx.x >= a.k) return;
   const int64_t c = load_int(a.ti, row * a.k + threadIdx.x, a.ti64);
-  const float t = load_any(a.tv, row * a.k + threadIdx.x, a.tv_type);
-  if (c >= 0 && c < a.V && !(t == -INFINITY)) {
+  const float v = load_any(a.tv, row * a.k + threadIdx.x, a.tv_type);
+  if (c >= 0 && c < a.V && !(v == -INFINITY)) {
     *cls = (int)c;
-    *u = (double)t * inv_t;
+    *t = v;
   }
 }
 
@@ -534,51 +584,68 @@ __device__ __forceinline__ void load_entry(const DistillArgs& a, int64_t row, do
 // once a piece.  Backward: the same pieces, read again and written; the named classes and the label
 // are written over afterwards by their own threads.  The gradient is not written by the forward: that
 // would save a pass only where the loss's own gradient is 1, and cost one (870 us for 600) elsewhere.
-// 4096 x 131072 in bf16 with the teacher's normaliser: forward 181 us (5.9 TB/s), backward 418 us (5.1
+// 4096 x 131072 in bf16 with the teacher's normaliser: forward 184 us (5.8 TB/s), backward 418 us (5.1
 // TB/s); 1023 x 50001 in fp16: 32 to 39 us and 40 us (rows of no alignment; 32 and 37 with rows of 50048).
+//
+// T^2 KD is of the logits' size at any T, so KD is of 1 / T^2, and what it is made of must not be
+// rounded at 1.  A row's sum of exponentials is held as S = n + e.  Up to T = kNearT n = 0 and e is a sum of
+// fp32 exponentials, joined in 64 bits; what they are rounded by reaches the loss T^2 times (a loss of 1
+// over 100 classes: 3e-7 at T = 4, 2e-6 at 8).  Above it n counts classes and e sums exp(z / T) - 1 in 64
+// bits, itself of 1 / T.  With log S = log n + log1p(e / n), and the teacher's sum the same way,
+// d_j = log p_j - log q_j is right to its last bits, and
+//   KD = sum_j (p_j d_j - p_j + q_j) + (r log(r / q_out) - r + q_out)
+// has no term below 0 and each of the order of d^2, so nothing cancels (without the rest's term what
+// p and q do not sum to is added as it is).  The gradients are q_j (exp(d_j) - 1) likewise, at any T.
+// Above kNearT the forward is bound by 64-bit arithmetic: 4096 x 131072 in bf16 680 us, 184 below; 4096 x
+// 1000 in fp32 47 us and 23.  The fp32 sums at T = 20 would be off by 1e-5, at 100 by 3e-4.
+constexpr double kNearT = 8.0;
 constexpr int kMaskWords = 4096;  // a thread's elements of a tile have one: 131,072 classes at a time, 65,536 of fp32
 
-// sums of a row's exponentials at T, and at 1 where the labels need it too, relative to one maximum
+// exponentials relative to the maximum m: their sum at T is n + e, at 1 (where the labels need it) s1
 struct Sums {
-  float m = kLowest, s = 0.f, s1 = 0.f;
-  __device__ __forceinline__ void merge(float om, float os, float os1, float c, float c1) {
-    const float n = fmaxf(m, om), a = m - n, b = om - n;
-    s = s * exp2_raw(a * c) + os * exp2_raw(b * c);
-    s1 = s1 * exp2_raw(a * c1) + os1 * exp2_raw(b * c1);
-    m = n;
+  float m = kLowest;
+  double n = 0, e = 0, s1 = 0;
+  // relative to another maximum, at or above m
+  __device__ __forceinline__ void move(float to, double inv_t) {
+    const double d = (double)m - to;
+    if (n > 0) e += expm1_neg(d * inv_t) * (n + e);
+    else e = e == 0 ? 0.0 : e * exp(d * inv_t);
+    s1 = s1 == 0 ? 0.0 : s1 * exp(d);
+    m = to;
   }
 };
 
-__device__ __forceinline__ Sums block_merge(Sums v, float c, float c1, float* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float om = __shfl_xor(v.m, o, 64), os = __shfl_xor(v.s, o, 64), os1 = __shfl_xor(v.s1, o, 64);
-    v.merge(om, os, os1, c, c1);
+// running sum of a thread's tiles, as TileSum, joined in 64 bits
+struct WideSum {
+  float m = kLowest, R = kLowest;
+  double s = 0;
+  __device__ __forceinline__ void raise(float top, float c) {
+    if (top > m) {
+      m = top;
+      const float n = fmaxf(top * c, kLowest);
+      s *= exp2_raw(R - n);
+      R = n;
+    }
   }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    float* r = red + 3 * (threadIdx.x >> 6);
-    r[0] = v.m;
-    r[1] = v.s;
-    r[2] = v.s1;
+  __device__ __forceinline__ float term(float z, float c) const { return exp2_raw(__builtin_fmaf(z, c, -R)); }
+  // what R was rounded by is taken back: for a small y, exp(-y) = 1 - y + y^2 / 2 to 2^-28
+  __device__ __forceinline__ double settled(float c) const {
+    const float x = __builtin_fmaf(m, c, -R);
+    const double y = x / kLog2e;
+    return !(s > 0) ? s : s * (fabsf(x) < 0x1p-9f ? 1.0 - y * (1.0 - 0.5 * y) : (double)exp2_raw(-x));
   }
-  __syncthreads();
-  Sums t;
-  for (int w = 0; w < kT / 64; ++w) t.merge(red[3 * w], red[3 * w + 1], red[3 * w + 2], c, c1);
-  return t;
-}
+};
 
-// classes [begin, end) of a row; `two`: both sums.  The mask has a word for each thread and tile, with
-// a bit for each of its elements.
-template <class T>
+// classes [begin, end) of a row; `two`: both sums; `masked`: without the named classes.  The mask has a
+// word for each thread and tile, with a bit for each of its elements.
+template <class T, bool FAR>
 __device__ __forceinline__ Sums row_sums(const DistillArgs& a, const typename T::store_t* z, int begin, int end,
-                                         int cls, bool two, uint32_t* mask, float* red) {
+                                         int cls, bool two, uint32_t* mask, double* red) {
   constexpr int N = Piece<T>::kN, TILE = kT * kU * N, kMasked = kMaskWords / kT * TILE;
   static_assert(kU * N <= 32, "a word has a bit for each of a thread's elements");
   const int tid = threadIdx.x;
   const float c = (float)(kLog2e / a.temperature), c1 = (float)kLog2e;
-  const bool tail = a.tlse != nullptr;
-  TileSum t, t1;
+  const bool masked = FAR || a.tlse != nullptr;
   auto word = [](int i) { return i / TILE * kT + i / N % kT; };
   auto bit = [](int i) { return i / (kT * N) % kU * N + i % N; };
   auto set_mask = [&](int v0, int n) {
@@ -588,79 +655,124 @@ __device__ __forceinline__ Sums row_sums(const DistillArgs& a, const typename T:
     if (cls >= v0 && cls < v0 + n) atomicOr(&mask[word(cls - v0)], 1u << bit(cls - v0));
     __syncthreads();
   };
-  for (int v0 = begin; v0 < end; v0 += kMasked) {
-    const int n = min(end - v0, kMasked);
-    if (tail) set_mask(v0, n);
-#pragma unroll 1
-    for (int base = 0; base < n; base += TILE) {
-      Piece<T> x[kU];
-      float f[kU * N];
-      load_tile<T, kT>(x, z + v0, base, n);
-#pragma unroll
-      for (int u = 0; u < kU; ++u)
-#pragma unroll
-        for (int e = 0; e < N; ++e) f[u * N + e] = x[u].get(e);
-      if (tail) {
-        const uint32_t bits = mask[base / TILE * kT + tid];
-        if (bits) {
-#pragma unroll
-          for (int e = 0; e < kU * N; ++e) f[e] = bits >> e & 1 ? -INFINITY : f[e];
-        }
-      }
-      float top = f[0], s = 0.f, s1 = 0.f;
-#pragma unroll
-      for (int e = 1; e < kU * N; ++e) top = fmaxf(top, f[e]);
-      t.raise(top, c);
-#pragma unroll
-      for (int e = 0; e < kU * N; ++e) s += t.term(f[e], c);
-      t.s += s;
-      if (two) {
-        t1.raise(top, c1);
-#pragma unroll
-        for (int e = 0; e < kU * N; ++e) s1 += t1.term(f[e], c1);
-        t1.s += s1;
-      }
-    }
-  }
-  Sums v;
-  v.m = t.m;
-  v.s = t.settled(c);
-  v.s1 = two ? t1.settled(c1) : 0.f;
-  v = block_merge(v, c, c1, red);
-  if (unsettled(v.m, v.s, c) || (two && unsettled(v.m, v.s1, c1))) {
-    MaxSum o, o1;
+  // f(a thread's elements of a tile), -inf for the named ones and behind the end
+  auto tiles = [&](auto f) {
     for (int v0 = begin; v0 < end; v0 += kMasked) {
       const int n = min(end - v0, kMasked);
-      if (tail) set_mask(v0, n);
-      for (int i = tid; i < n; i += kT) {
-        if (tail && (mask[word(i)] >> bit(i) & 1)) continue;
-        const float x = T::load(z[v0 + i]);
-        o.add(x, c);
-        if (two) o1.add(x, c1);
+      if (masked) set_mask(v0, n);
+#pragma unroll 1
+      for (int base = 0; base < n; base += TILE) {
+        Piece<T> x[kU];
+        float v[kU * N];
+        load_tile<T, kT, !FAR>(x, z + v0, base, n);
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[u * N + e] = x[u].get(e);
+        if (masked) {
+          const uint32_t bits = mask[base / TILE * kT + tid];
+          if (bits) {
+#pragma unroll
+            for (int e = 0; e < kU * N; ++e) v[e] = bits >> e & 1 ? -INFINITY : v[e];
+          }
+        }
+        f(v);
       }
     }
-    v.m = o.m;
-    v.s = o.s;
-    v.s1 = two ? o1.s : 0.f;
-    v = block_merge(v, c, c1, red);
+  };
+  Sums r;
+  if constexpr (FAR) {
+    // the maximum first (the row is read again, through the caches), then each class's deviation
+    float top = kLowest;
+    tiles([&](const float* v) {
+#pragma unroll
+      for (int e = 0; e < kU * N; ++e) top = fmaxf(top, v[e]);
+    });
+    r.m = block_max2(make_float2(top, kLowest), red).x;
+    const double inv_t = 1.0 / a.temperature;
+    int n = 0;
+    double s[3] = {0, 0, 0};
+    tiles([&](const float* v) {
+      float s1 = 0.f;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        bool some = false;
+#pragma unroll
+        for (int e = u * N; e < (u + 1) * N; ++e) some = some || v[e] != -INFINITY;
+        if (!__any(some)) continue;  // pieces behind the end of a short row
+#pragma unroll
+        for (int e = u * N; e < (u + 1) * N; ++e) {
+          const bool in = v[e] != -INFINITY;
+          const double x = expm1_neg(((double)v[e] - r.m) * inv_t);
+          n += in;
+          s[1] += in ? x : 0.0;
+          if (two) s1 += exp2_raw((v[e] - r.m) * c1);
+        }
+      }
+      s[2] += s1;
+    });
+    s[0] = n;
+    block_sums<3>(s, red);
+    r.n = s[0];
+    r.e = s[1];
+    r.s1 = s[2];
+  } else {
+    WideSum t, t1;
+    tiles([&](const float* v) {
+      float top = v[0], s = 0.f;
+#pragma unroll
+      for (int e = 1; e < kU * N; ++e) top = fmaxf(top, v[e]);
+      t.raise(top, c);
+#pragma unroll
+      for (int e = 0; e < kU * N; ++e) s += t.term(v[e], c);
+      t.s += s;
+      if (two) {
+        float s1 = 0.f;
+        t1.raise(top, c1);
+#pragma unroll
+        for (int e = 0; e < kU * N; ++e) s1 += t1.term(v[e], c1);
+        t1.s += s1;
+      }
+    });
+    auto join = [&](float m, double s, double s1) {
+      r.m = block_max2(make_float2(m, kLowest), red).x;
+      double v[2] = {s * exp2_raw((m - r.m) * c), s1 * exp2_raw((m - r.m) * c1)};
+      block_sums<2>(v, red);
+      r.e = v[0];
+      r.s1 = v[1];
+    };
+    join(t.m, t.settled(c), two ? t1.settled(c1) : 0.0);
+    if (unsettled(r.m, r.e, c) || (two && unsettled(r.m, r.s1, c1))) {
+      MaxSum o, o1;
+      for (int v0 = begin; v0 < end; v0 += kMasked) {
+        const int n = min(end - v0, kMasked);
+        if (masked) set_mask(v0, n);
+        for (int i = tid; i < n; i += kT) {
+          if (masked && (mask[word(i)] >> bit(i) & 1)) continue;
+          const float x = T::load(z[v0 + i]);
+          o.add(x, c);
+          if (two) o1.add(x, c1);
+        }
+      }
+      join(o.m, o.s, two ? o1.s : 0.f);
+    }
   }
-  return v;
+  return r;
 }
 
 struct RowShared {
-  float red[3 * kT / 64];
-  double redd[kT / 64];
+  double red[4 * kT / 64];
   int cls[kT];
 };
 
 // the row's named entry of this thread, the label, whether the row counts (block-wide)
 struct RowEntry {
   int cls;
-  double u;
+  float t;
   bool any, counted;
   int64_t y;
   __device__ __forceinline__ RowEntry(const DistillArgs& a, int64_t row, RowShared& sh) {
-    load_entry(a, row, 1.0 / a.temperature, &cls, &u);
+    load_entry(a, row, &cls, &t);
     sh.cls[threadIdx.x] = cls;
     any = __syncthreads_or(cls >= 0);
     y = a.target ? load_int(a.target, row, a.target64) : -1;
@@ -668,83 +780,126 @@ struct RowEntry {
   }
 };
 
+// What the backward needs of a row, in its kDistillStats floats.  A class outside the named ones gets
+// co exp((z - ref) / T) + h1 exp(z - top).  Of a named class q = ci exp((z - top) / T), with the weight
+// w = (1 - h) T in it, and an entry of it has p = w exp((t - tref) / T - norm) and, for its p / q,
+// log(p / q) = ((t - tref) - (z - top)) / T + K.  over: what p and the rest sum to, less 1.
+struct RowStats {
+  float ref, co, top, ci, h1, used, tref, over;
+  double norm, K;
+};
+static_assert(sizeof(RowStats) == kDistillStats * sizeof(float), "a row's statistics");
+
 // the row's loss and what its backward needs, from the sums over the classes outside the named ones
-// (with the teacher's lse) or over all
-template <class T>
+// (FAR, or with the teacher's lse) or over all
+template <class T, bool FAR>
 __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, const typename T::store_t* z,
-                                           const RowEntry& r, const Sums& out, RowShared& sh, float* loss_rows) {
+                                           const RowEntry& r, Sums out, RowShared& sh, float* loss_rows) {
   const int tid = threadIdx.x;
   const double inv_t = 1.0 / a.temperature;
-  const float c = (float)(kLog2e * inv_t), c1 = (float)kLog2e;
-  const bool tail = a.tlse != nullptr, two = a.hard > 0 && a.temperature != 1.0;
-  float* st = a.stats + row * kDistillStats;
-  const float zc = r.cls >= 0 ? T::load(z[r.cls]) : 0.f;
-  // all classes: those outside and the named ones, each class once.  Added in 64 bits, so the shares of
-  // the two sets are as near to each other as their sums say.
-  const bool has_out = out.s > 0.f || out.s != out.s;
-  float top = out.m;
-  double all_s = out.s, all_s1 = out.s1;
-  if (tail) {
-    bool first = r.cls >= 0;
+  const bool tail = a.tlse != nullptr, masked = FAR || tail, two = a.hard > 0 && a.temperature != 1.0;
+  const bool mine = r.cls >= 0, has_out = out.n > 0 || out.e > 0 || out.e != out.e;
+  const float zc = mine ? T::load(z[r.cls]) : 0.f;
+  bool first = mine;  // this entry is its class's first
+  if (masked) {
     for (int j = 0; j < a.k; j += 8) {  // threads without an entry hold -1
 #pragma unroll
       for (int e = 0; e < 8; ++e) first = first && (j + e >= tid || sh.cls[j + e] != r.cls);
     }
-    Sums in;
-    if (first && !(zc < kLowest)) {
-      in.m = zc == zc ? zc : kLowest;
-      in.s = in.s1 = zc == zc ? 1.f : zc;
+  }
+  RowStats st = {};
+  const float2 most = block_max2(make_float2(masked && mine ? zc : kLowest, mine ? r.t : kLowest), sh.red);
+  st.top = fmaxf(out.m, most.x);
+  st.tref = tail || !r.any ? 0.f : most.y;
+  // Waves without an entry only meet the others at the sums.  An entry's exponents are dz / T and dt / T.
+  const bool busy = (tid & ~63) < a.k;
+  const double dz = (double)zc - st.top, dt = (double)r.t - st.tref;
+  const bool live = masked && first && zc != -INFINITY;
+  double v[4] = {0, 0, 0, 0}, xz = 0;
+  if (busy && mine) {
+    xz = FAR ? expm1_neg(dz * inv_t) : exp(dz * inv_t);
+    if (live) v[0] = xz;
+    if (live && two) v[1] = exp(dz);
+    if (!tail) v[2] = FAR ? expm1_neg(dt * inv_t) : exp(dt * inv_t);
+    // how many classes the entries name and how many entries there are, each at most 256
+    if (FAR) v[3] = (live ? 1.0 : 0.0) + 512.0;
+  }
+  if constexpr (FAR) block_sums<4>(v, sh.red);
+  else if (tail) block_sums<2>(v, sh.red);
+  else block_sums<1>(v + 2, sh.red);
+  const double own = out.n + out.e;  // the sum outside, relative to its own maximum
+  const double shift = ((double)out.m - st.top) * inv_t;
+  double q_out = 0, S = 0, s1 = 0, whole = 0, part = 0;  // log S = whole + part
+  if (busy) {
+    const double entries = FAR ? floor(v[3] / 512) : 0.0, in = FAR ? v[3] - 512 * entries : 0.0;
+    Sums all = out;
+    if (has_out && out.m != st.top) all.move(st.top, inv_t);
+    q_out = all.n + all.e;
+    all.n += in;
+    all.e += v[0];
+    s1 = all.s1 + v[1];
+    S = all.n + all.e;
+    // `whole` cancels where the teacher's sum has as many classes
+    if (FAR) whole = log(all.n);
+    part = FAR ? log1p(all.e / all.n) : log(S);
+    if (tail) {
+      st.norm = a.tlse[row];
+      st.K = whole + part - st.norm;
+    } else if (r.any) {
+      const double w0 = FAR ? log(entries) : 0.0, p0 = FAR ? log1p(v[2] / entries) : log(v[2]);
+      st.norm = w0 + p0;
+      st.K = (whole - w0) + (part - p0);
     }
-    in = block_merge(in, c, c1, sh.red);
-    top = fmaxf(out.m, in.m);
-    const double d = (double)out.m - top, e = (double)in.m - top;
-    all_s = out.s * exp(d * inv_t) + in.s * exp(e * inv_t);
-    if (two) all_s1 = out.s1 * exp(d) + in.s1 * exp(e);
   }
-  const double log_z = log(all_s);
-  // the teacher
-  double norm = 0;
-  if (tail) {
-    norm = a.tlse[row];
-  } else if (r.any) {
-    double most = r.cls >= 0 ? r.u : -INFINITY;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) most = fmax(most, __shfl_xor(most, o, 64));
-    __syncthreads();
-    if ((tid & 63) == 0) sh.redd[tid >> 6] = most;
-    __syncthreads();
-    for (int w = 0; w < kT / 64; ++w) most = fmax(most, sh.redd[w]);
-    norm = most + log(block_sum_d(r.cls >= 0 ? exp(r.u - most) : 0.0, sh.redd));
+  v[0] = v[1] = v[2] = v[3] = 0;
+  if (busy && mine) {
+    const double p = exp(dt * inv_t - st.norm), d = (dt - dz) * inv_t + st.K;
+    const double pd = p == 0 ? 0.0 : p * d;  // p = 0 has no term, whatever the student's value
+    v[0] = pd;
+    v[1] = p;
+    if constexpr (FAR) {
+      const double q = (1.0 + xz) / S, gain = gain_near(d);
+      const bool near = fabs(d) < 0.25;
+      v[0] = near ? q * gain : pd - p + q;
+      v[2] = near ? q * ((d - gain) / (1.0 - d)) : p - q;  // q (exp(d) - 1)
+      v[3] = first ? 0.0 : q;
+    }
   }
-  const double p = r.cls >= 0 ? exp(r.u - norm) : 0.0;
-  // p = 0 has no term, whatever the student's value
-  double kd = block_sum_d(p == 0 ? 0.0 : p * ((r.u - norm) - (((double)zc - top) * inv_t - log_z)), sh.redd);
-  const double named = tail ? block_sum_d(p, sh.redd) : 1.0;
+  if constexpr (FAR) block_sums<4>(v, sh.red);
+  else if (tail) block_sums<2>(v, sh.red);
+  else block_sums<1>(v, sh.red);
   if (tid != 0) return;
-  // exp2((z - ref) c) * co: what a class outside gets
-  double mass = tail ? named : r.any ? 1.0 : 0.0, rest = 0.0;
-  const double shift = ((double)out.m - top) * inv_t;
-  if (tail && has_out && !(named >= 1)) {
-    rest = 1.0 - named;
-    kd += rest * (log(rest) - (shift + log((double)out.s) - log_z));
-    mass = 1.0;
+  double kd = v[0], co = 0;  // co exp((z - ref) / T): what a class outside gets
+  const double h = a.hard, w = (1 - h) * a.temperature, sum_p = tail ? v[1] : r.any ? 1.0 : 0.0;
+  q_out = has_out ? q_out / S : 0.0;
+  if (tail && has_out && !(sum_p >= 1)) {
+    const double rest = 1 - sum_p, log_q_out = shift + log(own) - whole - part;
+    if constexpr (FAR) {
+      const double less = v[2] + v[3], x = -less / q_out;  // less = q_out - rest
+      kd += fabs(x) < 0.2 ? q_out * gain_near(log1p(x)) : rest * (log(rest) - log_q_out) - rest + q_out;
+      kd -= v[3];
+      co = less / own;
+    } else {
+      kd += rest * (log(rest) - log_q_out);
+      co = exp(shift) / S - rest / own;
+    }
+  } else {
+    if (FAR) kd += (sum_p - 1) + q_out - v[3];
+    if (tail) st.over = (float)(sum_p - 1);
+    co = has_out ? sum_p * exp(shift) / S : S > 0 ? 0.0 : __builtin_nan("");  // a row of -inf has no distribution
   }
-  const double co = has_out ? mass * exp(shift) / all_s - (tail ? rest / out.s : 0.0)
-                    : all_s > 0 ? 0.0 : __builtin_nan("");  // a row of -inf has no distribution
-  const float ref = has_out ? out.m : top;
-  const double h = a.hard, z1 = two ? all_s1 : all_s;
+  if (!r.any) kd = 0;
+  st.ref = has_out ? out.m : st.top;
   // a weight of 0 takes the term out, whatever the teacher says (KD is infinite where a named class is masked)
-  const double w = (1 - h) * a.temperature;
+  const double z1 = two ? s1 : S;
   double loss = w == 0 ? 0.0 : w * a.temperature * kd;
-  if (h > 0) loss += h * (log(z1) - ((double)T::load(z[r.y]) - top));
+  if (h > 0) loss += h * (log(z1) - ((double)T::load(z[r.y]) - st.top));
   loss_rows[row] = (float)loss;
-  st[0] = ref;
-  st[1] = (float)((w == 0 ? 0.0 : w * co) + (h > 0 && !two ? h * exp((double)ref - top) / z1 : 0.0));
-  st[2] = top;
-  st[3] = r.any && w != 0 ? (float)(w * mass / all_s) : 0.f;
-  st[4] = h > 0 ? (float)(h / z1) : 0.f;
-  st[5] = 1.f;
-  *reinterpret_cast<double*>(st + 6) = norm;  // all its bits: with a small T it is large, and u near it
+  st.co = (float)((w == 0 ? 0.0 : w * co) + (h > 0 && !two ? h * exp((double)st.ref - st.top) / z1 : 0.0));
+  st.ci = r.any && w != 0 ? (float)(w / S) : 0.f;
+  st.h1 = h > 0 ? (float)(h / z1) : 0.f;
+  st.used = 1.f;
+  reinterpret_cast<RowStats*>(a.stats)[row] = st;
 }
 
 __device__ __forceinline__ void leave_out(const DistillArgs& a, int64_t row, float* loss_rows) {
@@ -753,9 +908,10 @@ __device__ __forceinline__ void leave_out(const DistillArgs& a, int64_t row, flo
 }
 
 // part == nullptr: a block has the whole row; else [rows][nseg] sums of a segment each, for distill_join_k
-template <class T>
-__global__ __launch_bounds__(kT, 8) void distill_fwd_k(DistillArgs a, int nseg, int seglen, float* __restrict__ part,
-                                                    float* __restrict__ loss_rows) {
+template <class T, bool FAR>
+__global__ __launch_bounds__(kT, FAR ? 4 : 8) void distill_fwd_k(DistillArgs a, int nseg, int seglen,
+                                                                 double* __restrict__ part,
+                                                                 float* __restrict__ loss_rows) {
   __shared__ RowShared sh;
   __shared__ uint32_t mask[kMaskWords];
   const int64_t row = blockIdx.x / nseg;
@@ -767,19 +923,20 @@ __global__ __launch_bounds__(kT, 8) void distill_fwd_k(DistillArgs a, int nseg, 
     return;
   }
   const bool two = a.hard > 0 && a.temperature != 1.0;
-  const Sums out = row_sums<T>(a, z, seg * seglen, min(a.V, (seg + 1) * seglen), r.cls, two, mask, sh.red);
+  const Sums out = row_sums<T, FAR>(a, z, seg * seglen, min(a.V, (seg + 1) * seglen), r.cls, two, mask, sh.red);
   if (!part) {
-    finish_row<T>(a, row, z, r, out, sh, loss_rows);
+    finish_row<T, FAR>(a, row, z, r, out, sh, loss_rows);
   } else if (threadIdx.x == 0) {
-    float* p = part + (row * nseg + seg) * 3;
+    double* p = part + (row * nseg + seg) * 4;
     p[0] = out.m;
-    p[1] = out.s;
-    p[2] = out.s1;
+    p[1] = out.n;
+    p[2] = out.e;
+    p[3] = out.s1;
   }
 }
 
-template <class T>
-__global__ __launch_bounds__(kT) void distill_join_k(DistillArgs a, int nseg, const float* __restrict__ part,
+template <class T, bool FAR>
+__global__ __launch_bounds__(kT) void distill_join_k(DistillArgs a, int nseg, const double* __restrict__ part,
                                                      float* __restrict__ loss_rows) {
   __shared__ RowShared sh;
   const int64_t row = blockIdx.x;
@@ -788,13 +945,19 @@ __global__ __launch_bounds__(kT) void distill_join_k(DistillArgs a, int nseg, co
   if (!r.counted) return leave_out(a, row, loss_rows);
   Sums v;
   if ((int)threadIdx.x < nseg) {
-    const float* p = part + (row * nseg + threadIdx.x) * 3;
-    v.m = p[0];
-    v.s = p[1];
-    v.s1 = p[2];
+    const double* p = part + (row * nseg + threadIdx.x) * 4;
+    v.m = (float)p[0];
+    v.n = p[1];
+    v.e = p[2];
+    v.s1 = p[3];
   }
-  v = block_merge(v, (float)(kLog2e / a.temperature), (float)kLog2e, sh.red);
-  finish_row<T>(a, row, z, r, v, sh, loss_rows);
+  v.move(block_max2(make_float2(v.m, kLowest), sh.red).x, 1.0 / a.temperature);
+  double s[3] = {v.n, v.e, v.s1};
+  block_sums<3>(s, sh.red);
+  v.n = s[0];
+  v.e = s[1];
+  v.s1 = s[2];
+  finish_row<T, FAR>(a, row, z, r, v, sh, loss_rows);
 }
 
 // loss = the sum or mean of the rows' losses; the rows' weight goes behind their statistics
@@ -804,7 +967,7 @@ __global__ __launch_bounds__(1024) void distill_mean_k(const float* __restrict__
   double s = 0, n = 0;
   for (int64_t i = threadIdx.x; i < rows; i += 1024) {
     s += loss_rows[i];
-    n += stats[i * kDistillStats + 5];
+    n += reinterpret_cast<const RowStats*>(stats)[i].used;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -839,9 +1002,9 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
   const int64_t row = blockIdx.x / nseg;
   const int begin = (int)(blockIdx.x % nseg) * seglen, end = min(a.V, begin + seglen);
   const auto* z = static_cast<const typename T::store_t*>(a.z) + row * a.ldz;
-  const float* st = a.stats + row * kDistillStats;
+  const RowStats& st = reinterpret_cast<const RowStats*>(a.stats)[row];
   dz += row * a.V;
-  if (st[5] == 0.f) {  // a row that is left out: its logits are not looked at
+  if (st.used == 0.f) {  // a row that is left out: its logits are not looked at
     const Bytes16 zero = {{0, 0, 0, 0}};
     for (int i = begin + tid * N; i < end; i += kT * N) {
       if (i + N <= end) *reinterpret_cast<Bytes16*>(dz + i) = zero;
@@ -854,7 +1017,7 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
   const double inv_t = 1.0 / a.temperature;
   const float c = (float)(kLog2e * inv_t), c1 = (float)kLog2e;
   const bool two = a.hard > 0 && a.temperature != 1.0;
-  const float ref = st[0], co = st[1], m = st[2], ci = st[3], h1 = st[4];
+  const float ref = st.ref, co = st.co, m = st.top, ci = st.ci, h1 = st.h1;
   // without a share (co = 0) a named class above `ref` must not make a NaN of an overflow
   const float lim = co == 0.f ? 0.f : INFINITY;
   constexpr int TILE = kT * kU * N;
@@ -891,22 +1054,31 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
   if (past_caches) sweep(std::true_type{});
   else sweep(std::false_type{});
   int cls;
-  double u;
-  load_entry(a, row, inv_t, &cls, &u);
+  float t, v = 0.f, q = 0.f;
+  load_entry(a, row, &cls, &t);
   cls_s[tid] = cls;
-  const double norm = *reinterpret_cast<const double*>(st + 6);
-  p_s[tid] = cls >= 0 && a.hard < 1 ? (float)((1 - a.hard) * a.temperature * exp(u - norm)) : 0.f;
+  double less = 0;  // p - q of an entry
+  if (cls >= 0 && ci != 0.f) {
+    v = T::load(z[cls]);
+    q = ci * exp2f((v - m) * c);
+    const double dt = (double)t - st.tref, d = (dt - ((double)v - m)) * inv_t + st.K;
+    less = fabs(d) < 0.25 ? q * ((d - gain_near(d)) / (1.0 - d))
+                          : (1 - a.hard) * a.temperature * exp(dt * inv_t - st.norm) - q;
+  }
+  p_s[tid] = (float)less;
   const int64_t y = a.hard > 0 ? load_int(a.target, row, a.target64) : -1;
   __syncthreads();  // also orders the stores above before the ones below
   if (cls >= begin && cls < end) {
-    float p = 0;  // a class that is named twice has both entries' share
+    float more = 0, times = 0;  // a class that is named twice has both entries' share
     for (int j = 0; j < a.k; j += 8) {  // threads without an entry hold -1
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p += cls_s[j + e] == cls ? p_s[j + e] : 0.f;
+      for (int e = 0; e < 8; ++e) {
+        more += cls_s[j + e] == cls ? p_s[j + e] : 0.f;
+        times += cls_s[j + e] == cls ? 1.f : 0.f;
+      }
     }
-    const float v = T::load(z[cls]);
-    const float q = ci == 0.f ? 0.f : ci * exp2f((v - m) * c);
-    float d = q - p;
+    float d = ci == 0.f ? 0.f : q * (1.f - times + st.over) - more;
+    if (ci == 0.f) v = T::load(z[cls]);
     if (a.hard > 0) d += h1 * exp2f((v - m) * c1) - (cls == y ? (float)a.hard : 0.f);
     dz[cls] = T::store(g * d);
   }
@@ -959,20 +1131,25 @@ void top_logits(const void* z, int type, int64_t ldz, int64_t rows, int V, int k
 
 int64_t distill_scratch(int64_t rows, int V) {
   const int nseg = row_segments(rows, V);
-  return nseg > 1 ? 3 * rows * nseg : 0;
+  return nseg > 1 ? 8 * rows * nseg : 0;
 }
 
-void distill_fwd(const DistillArgs& a, float* loss_rows, float* loss, bool mean, float* scratch, hipStream_t st) {
+void distill_fwd(const DistillArgs& a, float* loss_rows, float* loss, bool mean, void* scratch, hipStream_t st) {
   check_distill(a);
   int nseg = row_segments(a.rows, a.V);
   const int seglen = segment_length(a.V, &nseg);
-  MX_CHECK(nseg == 1 || scratch, "distill_loss: long rows need scratch");
+  MX_CHECK(nseg == 1 || (scratch && (uintptr_t)scratch % 8 == 0), "distill_loss: long rows need scratch");
+  auto launch = [&](auto type, auto far) {
+    using T = decltype(type);
+    constexpr bool FAR = far.value;
+    double* part = nseg > 1 ? static_cast<double*>(scratch) : nullptr;
+    MX_LAUNCH((distill_fwd_k<T, FAR>), dim3((uint32_t)(a.rows * nseg)), dim3(kT), 0, st, a, nseg, seglen, part, loss_rows);
+    if (nseg > 1) MX_LAUNCH((distill_join_k<T, FAR>), dim3((uint32_t)a.rows), dim3(kT), 0, st, a, nseg, part, loss_rows);
+  };
   if (a.rows > 0)
     MX_BY_TYPE(a.type, T, {
-      MX_LAUNCH(distill_fwd_k<T>, dim3((uint32_t)(a.rows * nseg)), dim3(kT), 0, st, a, nseg, seglen,
-                nseg > 1 ? scratch : nullptr, loss_rows);
-      if (nseg > 1)
-        MX_LAUNCH(distill_join_k<T>, dim3((uint32_t)a.rows), dim3(kT), 0, st, a, nseg, scratch, loss_rows);
+      if (a.temperature > kNearT) launch(T{}, std::true_type{});
+      else launch(T{}, std::false_type{});
     });
   if (loss) MX_LAUNCH(distill_mean_k, dim3(1), dim3(1024), 0, st, loss_rows, a.stats, a.rows, mean ? 1 : 0, loss);
 }

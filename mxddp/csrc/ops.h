@@ -330,16 +330,16 @@ struct DistillArgs {
   const void* ti;       // [rows][k] their classes (outside [0, V): unused entry)
   const void* target;   // [rows] or null: the row's class (outside [0, V): row left out)
   const float* tlse;    // [rows] or null: the teacher's log sum exp(t / T) over all classes
-  float* stats;         // [rows * kDistillStats + 1], written by the forward, read by the backward
+  float* stats;         // [rows * kDistillStats + 1], at a multiple of 16 bytes, written by the forward, read by the backward
   int64_t ldz, rows;
   int V, k, type, tv_type, ti64, target64;
   double temperature, hard;
 };
-constexpr int kDistillStats = 8;
+constexpr int kDistillStats = 12;
 // loss_rows [rows]: each row's loss; loss (or null): their mean over the counted rows, or their sum
-// scratch: distill_scratch(...) floats (0: none needed)
+// scratch: distill_scratch(...) floats at a multiple of 8 bytes (0: none needed)
 int64_t distill_scratch(int64_t rows, int V);
-void distill_fwd(const DistillArgs& a, float* loss_rows, float* loss, bool mean, float* scratch, hipStream_t st);
+void distill_fwd(const DistillArgs& a, float* loss_rows, float* loss, bool mean, void* scratch, hipStream_t st);
 // dz [rows][V] = dloss * d loss / dz; dloss: one value, or per_row one for each row's loss
 void distill_bwd(const DistillArgs& a, const float* dloss, bool per_row, void* dz, hipStream_t st);
 

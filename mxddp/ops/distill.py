@@ -19,6 +19,7 @@ from .lowp import DTYPES, MAX_ROWS, check_device, check_float, has_derivative, o
 
 MAX_TOP = 256       # csrc/ops.h kTopMax
 MAX_CLASSES = 2**30
+_STATS = 12         # csrc/ops.h kDistillStats
 
 
 class TopLogits(NamedTuple):
@@ -82,15 +83,16 @@ class _DistillLoss(torch.autograd.Function):
         C, (rows, V) = native(), z.shape
         # the rows' statistics and weight for the backward, then what is used up here: the rows'
         # losses (the result itself without a reduction) and the sums of a split row
-        n = 8 * rows + 1
-        buf = torch.empty((n + rows + C.distill_scratch(rows, V),), device=z.device, dtype=torch.float32)
+        n = _STATS * rows + 1
+        spare = (n + rows + 1) // 2 * 2  # 64-bit sums
+        buf = torch.empty((spare + C.distill_scratch(rows, V),), device=z.device, dtype=torch.float32)
         loss = torch.empty(() if reduction != "none" else (rows,), device=z.device, dtype=torch.float32)
         per_row = reduction == "none"
         p = buf.data_ptr()
         with on_device(z):
             C.distill_fwd(*_args(z, tv, ti, target, tlse, buf, temperature, hard),
                           loss.data_ptr() if per_row else p + 4 * n, 0 if per_row else loss.data_ptr(),
-                          reduction == "mean", p + 4 * (n + rows), stream(z))
+                          reduction == "mean", p + 4 * spare, stream(z))
         ctx.save_for_backward(z, tv, ti, target, tlse, buf)
         ctx.args = (temperature, hard)
         ctx.per_row = per_row
@@ -108,31 +110,79 @@ class _DistillLoss(torch.autograd.Function):
         return dz, None, None, None, None, None, None, None
 
 
+def _gain(d):
+    """x e^x - e^x + 1 = sum x^n (n - 1) / n!, for |x| <= 1/4 without the difference of near numbers."""
+    near = d.abs() < 0.25
+    x = torch.where(near, d, 0.0)
+    series = torch.zeros_like(x)
+    for n in range(14, 1, -1):
+        series = series * x + (n - 1) / math.factorial(n)
+    x = torch.where(near, 0.0, d)
+    return torch.where(near, series * torch.where(near, d, 0.0) ** 2, x * x.exp() - torch.expm1(x))
+
+
 def _distill_kd(z, tv, ti, tlse, temperature, used, counted):
-    """Each row's KL(p || q), in 64 bits."""
-    V = z.shape[1]
+    """Each row's KL(p || q), in 64 bits; of size 1 / T^2 and right to its last digits at any T: sums of
+    exponentials are held by how far they are from the number of their terms, and what is added up has
+    no negative part (``csrc/distill.hip``)."""
+    V, k = z.shape[1], tv.shape[1]
     at = torch.where(used, ti, 0).long()
-    zt = z / temperature
-    total = torch.logsumexp(zt, 1)
-    u = torch.where(used, tv.double() / temperature, -math.inf)
+    slot = torch.where(used, at, V)
+    place = torch.arange(k, device=z.device, dtype=torch.int32).expand(ti.shape)
+    first = torch.full((z.shape[0], V + 1), k, dtype=torch.int32, device=z.device).scatter_reduce_(1, slot, place, "amin")
+    named = first[:, :V] < k
+    first = used & (first.gather(1, slot) == place)  # an entry that is its class's first
+    # the student
+    live = z.detach() != -math.inf
+    top = z.detach().amax(1, keepdim=True)
+    dz = z - torch.where(live.any(1, keepdim=True), top, 0.0)
+    n, e = live.sum(1).double(), torch.where(live, torch.expm1(dz.detach() / temperature), 0.0).sum(1)
+    whole, part = n.log(), torch.log1p(e / n)  # of log sum exp(dz / T); its derivative is logsumexp's
+    total = torch.logsumexp(dz / temperature, 1)
+    part = part + (total - total.detach())
+    share = torch.softmax(dz / temperature, 1)
+    # the teacher
+    tv = tv.double()
     if tlse is not None:
+        dt = torch.where(used, tv, 0.0)
         norm = torch.where(counted, tlse.double(), 0.0)
+        log_ratio = whole + part - norm
     else:
-        norm = torch.logsumexp(u, 1)
-        norm = torch.where(used.any(1), norm, 0.0)
-    logp = u - norm[:, None]
-    p = logp.exp()
-    term = torch.where(p != 0, logp, 0.0) - (zt.gather(1, at) - total[:, None])
-    kd = torch.where(p != 0, p * torch.where(p != 0, term, 0.0), 0.0).sum(1)
+        most = torch.where(used, tv, -math.inf).amax(1, keepdim=True)
+        dt = torch.where(used, tv - most, 0.0)
+        m = used.sum(1).double()
+        p1 = torch.log1p(torch.where(used, torch.expm1(dt / temperature), 0.0).sum(1) / m)
+        norm = m.log() + p1
+        log_ratio = (whole - m.log()) + (part - p1)
+    p = torch.where(used, (dt / temperature - norm[:, None]).exp(), 0.0)
+    q = torch.where(used, share.gather(1, at), 0.0)
+    d = (dt - dz.gather(1, at)) / temperature + log_ratio[:, None]  # log p - log q
+    has_p = used & (p != 0)
+    near = has_p & (d.detach().abs() < 0.25)
+    far = torch.where(has_p & ~near, p * torch.where(has_p & ~near, d, 0.0), 0.0) - p + q
+    kd = torch.where(near, q * _gain(torch.where(near, d, 0.0)), far).sum(1)
+    less = torch.where(near, q * torch.expm1(torch.where(near, d, 0.0)), p - q).sum(1)  # sum p - sum q
+    twice = torch.where(first, 0.0, q).sum(1)
+    q_out = torch.where(live & ~named, share, 0.0).sum(1)
+    rest = torch.zeros_like(kd)
+    sum_p = torch.ones_like(kd)
     if tlse is not None:
-        named = torch.zeros(z.shape[0], V + 1, dtype=torch.bool, device=z.device)
-        named = named.scatter_(1, torch.where(used, at, V), True)[:, :V]
-        rest = (1 - p.sum(1)).clamp_min(0)
-        has = (rest != 0) & ((zt.detach() > -math.inf) & ~named).any(1)
-        outside = torch.logsumexp(torch.where(named & has[:, None], -math.inf, zt), 1)
-        safe = torch.where(has, rest, 1.0)
-        kd = kd + torch.where(has, safe * (safe.log() - (outside - total)), 0.0)
-    return torch.where(used.any(1), kd, 0.0) if tlse is None else kd
+        sum_p = p.sum(1)
+        has = (live & ~named).any(1) & ~(sum_p >= 1)
+        q_safe = torch.where(has & (q_out != 0), q_out, 1.0)
+        over = -(less + twice) / q_safe  # rest / q_out - 1
+        by_sum = (over.detach().abs() < 0.2) & (q_out.detach() != 0)
+        rest = torch.where(has, 1 - sum_p, 0.0)
+        r = torch.where(has, rest, 1.0)
+        # log q_out, also where it is too small for a number
+        out = torch.where(live & ~named, dz / temperature, -math.inf)
+        log_q = torch.logsumexp(torch.where(has[:, None], out, 0.0), 1) - whole - part
+        gain = torch.where(by_sum, q_out * _gain(torch.log1p(torch.where(by_sum, over, 0.0))),
+                           r * (r.log() - log_q) - r + q_out)
+        rest = torch.where(has, gain, (sum_p - 1) + q_out)
+    else:
+        rest = q_out
+    return torch.where(used.any(1), kd + rest - twice, 0.0)
 
 
 def _distill_rows(z, tv, ti, target, tlse, temperature, hard):

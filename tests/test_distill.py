@@ -9,6 +9,7 @@ chain and 64 steps of joining (each with an exponential that rescales).  So s is
 most ES = (V / 64 + 64 + 3 log V + 4) E, and log s by that much absolutely.
 """
 import math
+from decimal import Decimal, localcontext
 
 import pytest
 import torch
@@ -386,6 +387,142 @@ def test_distill_loss_small_shares(dev, V, k, T):
     tv, ti, lse = ops.top_logits(teacher, k, T)
     check_distill(dev, z, tv, ti, None, lse, T)
     check_distill(dev, z, tv, ti, None, lse, T, 0.0, "none")
+
+
+def oracle_decimal(z, tv, ti, target, tlse, T, h):
+    """One row's loss and gradient from the formulas, in 160 digits, and the shares q and softmax(z)."""
+    with localcontext() as c:
+        c.prec = 160
+        zero, one, T, w1 = Decimal(0), Decimal(1), Decimal(T), Decimal(1) - Decimal(h)
+        z = [Decimal(v) if v != -INF else None for v in z]
+        lse = lambda v: (lambda m: m + sum((x - m).exp() for x in v).ln())(max(v))  # noqa: E731
+        zt = [None if v is None else v / T for v in z]
+        total = lse([v for v in zt if v is not None])
+        q = [zero if v is None else (v - total).exp() for v in zt]
+        pairs = [(int(i), Decimal(v) / T) for i, v in zip(ti, tv) if 0 <= i < len(z) and v != -INF]
+        norm = lse([u for _, u in pairs]) if tlse is None else Decimal(tlse)
+        p = [(i, (u - norm).exp()) for i, u in pairs]
+        mass = sum((x for _, x in p), zero)
+        kd = sum((x * (u - norm - (zt[i] - total)) for (i, x), (_, u) in zip(p, pairs)), zero)
+        out = [i for i in range(len(z)) if z[i] is not None and i not in {i for i, _ in p}]
+        share, rest, q_out = mass, zero, sum((q[i] for i in out), zero)
+        if tlse is not None and out and mass < 1:
+            rest, share = one - mass, one
+            kd += rest * (rest.ln() - q_out.ln())
+        grad = [share * x for x in q]
+        for i in out:
+            if rest > 0:
+                grad[i] -= rest * q[i] / q_out
+        for i, x in p:
+            grad[i] -= x
+        loss, grad = w1 * T * T * kd, [w1 * T * g for g in grad]
+        soft = [0.0] * len(z)
+        if h > 0:
+            l1 = lse([v for v in z if v is not None])
+            loss += Decimal(h) * (l1 - z[target])
+            for i, v in enumerate(z):
+                if v is not None:
+                    soft[i] = float((v - l1).exp())
+                    grad[i] += Decimal(h) * (v - l1).exp()
+            grad[target] -= Decimal(h)
+        return float(loss), [float(g) for g in grad], [float(x) for x in q], soft
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("N,V,k,kind,T", [(3, 10, 10, "all", T) for T in (8.5, 20.0, 100.0, 1e4, 1e6, 1e12, 1e30)]
+                         + [(3, 100, 40, "few", T) for T in (8.5, 20.0, 100.0, 1e4, 1e6, 1e12, 1e30)]
+                         + [(2, 256, 256, "all", T) for T in (20.0, 1e6)] + [(3, 100, 40, "near", T) for T in (9.0, 1e4)]
+                         + [(2, 200, 30, "masked", T) for T in (10.0, 1e3)] + [(2, 120, 24, "twice", T) for T in (20.0, 1e5)]
+                         + [(1, 8200, 64, "few", T) for T in (12.0, 1e6)])
+@pytest.mark.parametrize("tail,h", [(False, 0.0), (True, 0.0), (True, 0.3)])
+def test_distill_loss_high_temperatures(dev, N, V, k, kind, T, tail, h):
+    """T^2 KL keeps the size of the logits' differences at any T, and so does its gradient times 1 / T: with
+    e the distance of two logarithms log p - log q (each right to a few steps U = 2^-53 of its parts, the
+    sums of exponentials to (V / 64 + 64) U of how far their terms are from 1), KL is made of terms p e, each
+    paired with its share so that none is negative, and the gradient of terms q (exp(e) - 1)."""
+    dtype = TYPES[(N + V) % 3]
+    g = torch.Generator().manual_seed(V + k)
+    teacher = (3 * torch.randn(N, V, generator=g)).to(dtype)
+    noise = 0.01 if kind == "near" else 1.0
+    z = (teacher.float() * (1.0 if kind == "near" else 0.5) + noise * torch.randn(N, V, generator=g)).to(dtype)
+    tv, ti = (t[:, :k].contiguous() for t in torch.sort(teacher, dim=1, descending=True))
+    if kind == "masked":
+        z[:, torch.randperm(V, generator=g)[:50]] = -INF
+        z.scatter_(1, ti, tv - 1)
+        ti[0, 3], tv[1, 5] = -1, -INF
+    if kind == "twice":
+        ti[:, 4], ti[:, 9], ti[:, 10] = ti[:, 1], ti[:, 2], ti[:, 2]
+    lse = torch.logsumexp(teacher.double() / T, 1).float() if tail else None
+    y = torch.arange(N) + 2 if h else None
+    if h:
+        z.scatter_(1, y[:, None], torch.where(z.gather(1, y[:, None]) == -INF, 0.0, z.gather(1, y[:, None])))
+    leaf = z.to(dev, copy=True).requires_grad_()
+    loss = ops.distill_loss(leaf, tv.to(dev), ti.to(dev), None if y is None else y.to(dev),
+                            None if lse is None else lse.to(dev), T, h, "none")
+    grad, = torch.autograd.grad(loss.sum(), leaf)
+    fi = torch.finfo(dtype)
+    for r in range(N):
+        want, wg, q, soft = oracle_decimal(z[r].tolist(), tv[r].tolist(), ti[r].tolist(), None if y is None else int(y[r]),
+                                           None if lse is None else lse[r].item(), T, h)
+        zr = z[r][z[r] != -INF].double()
+        gap = float(zr.max() - zr.min() + tv[r][tv[r] != -INF].double().max() - tv[r][tv[r] != -INF].double().min())
+        high = gap if not tail else float(max(gap, tv[r][tv[r] != -INF].double().abs().max()))
+        U = 2.0**-53 * 8 * (V / 64 + 64)
+        ends = abs(lse[r].item()) + math.log(V) if tail else 0.0  # what does not shrink with 1 / T
+        d = U * (high / T + ends)  # of one log p - log q
+        largest = 2 * gap / T + (E * ends if tail else 0.0)  # how far apart p and q are
+        tol = 2 * E * abs(want) + T * T * (d * largest + d * d) + h * es(V)
+        got = loss[r].item()
+        if abs(want) > 3.4e38:
+            assert got == math.copysign(INF, want)
+        else:
+            assert abs(got - want) <= tol, (got, want, tol)
+            if h == 0 and T <= (100 if tail else 1e6) and kind != "twice":  # the bound is far below the loss
+                assert tol < 1e-3 * abs(want)
+        wg, q, soft = (torch.tensor(v, dtype=torch.float64) for v in (wg, q, soft))
+        far = (zr.max() - z[r].double()).clamp_max(1e300) / T
+        hard = h * times(soft, es(V) + 4 * E * (far * T + 2)) + (4 * E * h if h else 0.0)
+        tg = (16 + 8 * gap / T) * E * (wg.abs() + h * (soft + 1)) + T * q * d * 4 + hard
+        if kind == "twice":  # two shares of one class side by side
+            tg = tg + 16 * E * T * q
+        tg = tg + fi.eps / 2 * 1.01 * (wg.abs() + tg) + fi.smallest_normal * fi.eps + 2.0**-126 * (2 * T + h)
+        gr = grad[r].cpu().double()
+        big = wg.abs() > fi.max
+        assert bool(((gr - wg).abs() <= tg)[~big].all()), float(((gr - wg).abs() / tg)[~big].max())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("V,k,T", [(300, 2, 4.0), (50000, 1, 4.0), (50000, 40, 8.0), (4096, 20, 1.0), (50000, 40, 30.0)])
+def test_distill_loss_small_losses(dev, V, k, T):
+    """A student near its teacher and classes that hold little, against bounds far below the loss and the
+    gradients.  An error of the sum S outside the named classes moves KD by (q_out - rest) d log S to first
+    order and q_in q_out / 2 d log S^2 to second; log S is right to EO = (32 + 3 (V / 4096 + 1) + 3 log V + 8) E: a tile's 32
+    terms added up in fp32, its rescaling at each of a thread's V / 4096 + 1 tiles, the exponents' three
+    roundings and the exponential's; what is joined after that is in 64 bits."""
+    g = torch.Generator().manual_seed(V + int(T))
+    teacher = torch.randn(4, V, generator=g)
+    z = teacher + 0.05 * torch.randn(4, V, generator=g)
+    tv, ti, lse = ops.top_logits(teacher, k, T)
+    leaf = z.to(dev, copy=True).requires_grad_()
+    loss = ops.distill_loss(leaf, tv.to(dev), ti.to(dev), top_lse=lse.to(dev), temperature=T, reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), leaf)
+    rows, _, wg, _, _ = oracle(z, tv, ti, None, lse, T, 0.0)
+    eo = (32 + 3 * (V / 4096 + 1) + 3 * math.log(V + 1) + 8) * E
+    q = torch.softmax(z.double() / T, 1)
+    named = torch.zeros(4, V, dtype=torch.bool).scatter_(1, ti.long(), True)
+    p = (tv.double() / T - lse.double()[:, None]).exp()
+    rest, q_out = 1 - p.sum(1), torch.where(named, 0.0, q).sum(1)
+    tol = T * T * (eo * (q_out - rest).abs() + eo * eo * (1 - q_out) + 2.0**-50 * math.log(V)) + 2 * E * rows
+    assert bool((tol < 0.1 * rows).all()), (tol / rows).max()
+    assert bool(((loss.detach().cpu().double() - rows).abs() <= tol).all())
+    # a named class: q (exp(d) - 1) with d right to EO; one outside: q / q_out times (q_out - rest), right to
+    # EO q_in q_out
+    q_in = 1 - q_out
+    tg = T * torch.where(named, q * eo, q / q_out[:, None] * (eo * q_in * q_out)[:, None]) + 16 * E * wg.abs()
+    tg = tg + T * q * 2.0**-50 * math.log(V) + 2.0**-148 + 2.0**-126 * 2 * T
+    assert bool((tg[named] < 0.05 * wg[named].abs().median()).all())
+    assert bool((tg[~named] < 0.5 * wg[~named].abs()).all()), (tg / wg.abs())[~named].max()
+    assert bool(((grad.cpu().double() - wg).abs() <= tg).all())
 
 
 @pytest.mark.parametrize("dev", DEVICES)
