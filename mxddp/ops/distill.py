@@ -197,7 +197,9 @@ def _distill_rows(z, tv, ti, target, tlse, temperature, hard):
         loss = (1 - hard) * temperature * temperature * _distill_kd(z, tv, ti, tlse, temperature, used, counted)
     if hard > 0:
         y = torch.where(counted, target, 0).long()[:, None]
-        loss = loss + hard * (torch.logsumexp(z, 1) - z.gather(1, y)[:, 0])
+        top = z.detach().amax(1, keepdim=True)
+        dz = z - torch.where(torch.isfinite(top), top, 0.0)  # a row of the type's lowest value keeps its log V
+        loss = loss + hard * (torch.logsumexp(dz, 1) - dz.gather(1, y)[:, 0])
     return torch.where(counted, loss, 0.0), counted
 
 
@@ -252,8 +254,8 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torc
                          f"{tuple(top_lse.shape)}")
     for t, name in ((top_values, "top_values"), (top_index, "top_index"), (target, "target"), (top_lse, "top_lse")):
         check_device(t, logits, name)
-        if has_derivative(t):
-            raise ValueError(f"distill_loss: {name} gets no gradient; detach it")
+    if has_derivative(top_values, top_lse):
+        raise ValueError("distill_loss: top_values and top_lse get no gradient; detach them")
     temperature, hard = _check_temperature(temperature), float(hard_weight)
     if not 0 <= hard <= 1:
         raise ValueError(f"distill_loss: hard_weight must be within 0 .. 1, got {hard_weight}")
@@ -266,10 +268,9 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torc
     tlse = None if top_lse is None else top_lse.reshape(-1)
     if not _native(logits):
         loss, counted = _distill_rows(z, tv, ti, target, tlse, temperature, hard)
-        loss = loss if logits.dtype == torch.float64 else loss.float()
-        if reduction == "none":
-            return loss.reshape(lead)
-        return loss.sum() / counted.sum().clamp_min(1) if reduction == "mean" else loss.sum()
+        loss = loss.reshape(lead) if reduction == "none" else loss.sum()
+        loss = loss / counted.sum().clamp_min(1) if reduction == "mean" else loss
+        return loss if logits.dtype == torch.float64 else loss.float()
     if z.shape[0] > MAX_ROWS:
         raise ValueError(f"distill_loss: {z.shape[0]} rows, at most {MAX_ROWS}")
     loss = _DistillLoss.apply(z, tv.contiguous(), ti.contiguous(), None if target is None else target.contiguous(),

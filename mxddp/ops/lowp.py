@@ -23,10 +23,13 @@ def check_device(t: torch.Tensor | None, x: torch.Tensor, name: str) -> None:
 def has_derivative(*tensors: torch.Tensor | None) -> bool:
     """Whether autograd would carry a derivative through any of these: backward while it records, or a
     forward-mode tangent (which torch.no_grad does not turn off)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
-                                                  for t in tensors)
+    backward, forward = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    if backward or forward:
+        for t in tensors:
+            if t is not None and (backward and t.requires_grad
+                                  or forward and forward_ad.unpack_dual(t).tangent is not None):
+                return True
+    return False
 
 
 def rows_of(t: torch.Tensor) -> torch.Tensor:

@@ -405,14 +405,15 @@ def oracle_decimal(z, tv, ti, target, tlse, T, h):
         mass = sum((x for _, x in p), zero)
         kd = sum((x * (u - norm - (zt[i] - total)) for (i, x), (_, u) in zip(p, pairs)), zero)
         out = [i for i in range(len(z)) if z[i] is not None and i not in {i for i, _ in p}]
-        share, rest, q_out = mass, zero, sum((q[i] for i in out), zero)
+        share, rest = mass, zero
         if tlse is not None and out and mass < 1:
             rest, share = one - mass, one
-            kd += rest * (rest.ln() - q_out.ln())
+            outside = lse([zt[i] for i in out])
+            kd += rest * (rest.ln() - (outside - total))
         grad = [share * x for x in q]
         for i in out:
             if rest > 0:
-                grad[i] -= rest * q[i] / q_out
+                grad[i] -= rest * (zt[i] - outside).exp()
         for i, x in p:
             grad[i] -= x
         loss, grad = w1 * T * T * kd, [w1 * T * g for g in grad]
@@ -523,6 +524,30 @@ def test_distill_loss_small_losses(dev, V, k, T):
     assert bool((tg[named] < 0.05 * wg[named].abs().median()).all())
     assert bool((tg[~named] < 0.5 * wg[~named].abs()).all()), (tg / wg.abs())[~named].max()
     assert bool(((grad.cpu().double() - wg).abs() <= tg).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1.0, 4.0, 20.0])
+def test_distill_loss_rows_of_one_value(dev, dtype, T):
+    """Rows that hold one value everywhere, the type's lowest, its largest and others: the student knows
+    nothing, the labels' loss is log V whatever the value, and so is KL to a teacher that is sure."""
+    V = 24
+    low, big = torch.finfo(dtype).min, torch.finfo(dtype).max
+    z = torch.tensor([low, big, 0.0, -1e4, 3e4]).to(dtype)[:, None].expand(5, V)
+    tv, ti = torch.tensor([[1e4, -3e4]]).to(dtype).expand(5, 2), torch.tensor([[3, 7]]).expand(5, 2)
+    y = torch.full((5,), 7)
+    leaf = z.to(dev, copy=True).requires_grad_()
+    for h in (0.0, 0.5, 1.0):
+        loss = ops.distill_loss(leaf, tv.to(dev), ti.to(dev), y.to(dev), None, T, h, "none")
+        g, = torch.autograd.grad(loss.sum(), leaf)
+        want = (h + (1 - h) * T * T) * math.log(V)
+        assert bool(((loss.detach().cpu().double() - want).abs() <= (h + (1 - h) * T * T) * es(V) + 2 * E * want).all())
+        wg = torch.full((V,), (h + (1 - h) * T) / V, dtype=torch.float64)
+        wg[3] -= (1 - h) * T
+        wg[7] -= h
+        tol = es(V) * (h + (1 - h) * T) + torch.finfo(dtype).eps / 2 * 1.01 * wg.abs() + 2.0**-24
+        assert bool(((g.cpu().double() - wg).abs() <= tol).all())
 
 
 @pytest.mark.parametrize("dev", DEVICES)
