@@ -781,11 +781,11 @@ struct RowEntry {
 };
 
 // What the backward needs of a row, in its kDistillStats floats.  A class outside the named ones gets
-// co exp((z - ref) / T) + h1 exp(z - top).  Of a named class q = ci exp((z - top) / T), with the weight
-// w = (1 - h) T in it, and an entry of it has p = w exp((t - tref) / T - norm) and, for its p / q,
-// log(p / q) = ((t - tref) - (z - top)) / T + K.  over: what p and the rest sum to, less 1.
+// co exp((z - ref) / T) + h1 exp(z - top).  A named class has q = ci exp((z - top) / T), with the weight
+// w = (1 - h) T in it and what p and the rest sum to; an entry of it has p = w exp((t - tref) / T - norm),
+// and log(p / q) = ((t - tref) - (z - top)) / T + K.
 struct RowStats {
-  float ref, co, top, ci, h1, used, tref, over;
+  float ref, co, top, ci, h1, used, tref, unused;
   double norm, K;
 };
 static_assert(sizeof(RowStats) == kDistillStats * sizeof(float), "a row's statistics");
@@ -869,7 +869,7 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, co
   else if (tail) block_sums<2>(v, sh.red);
   else block_sums<1>(v, sh.red);
   if (tid != 0) return;
-  double kd = v[0], co = 0;  // co exp((z - ref) / T): what a class outside gets
+  double kd = v[0], co = 0, mass = 1;  // co exp((z - ref) / T): what a class outside gets
   const double h = a.hard, w = (1 - h) * a.temperature, sum_p = tail ? v[1] : r.any ? 1.0 : 0.0;
   q_out = has_out ? q_out / S : 0.0;
   if (tail && has_out && !(sum_p >= 1)) {
@@ -885,7 +885,8 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, co
     }
   } else {
     if (FAR) kd += (sum_p - 1) + q_out - v[3];
-    if (tail) st.over = (float)(sum_p - 1);
+    mass = sum_p;
+    if (tail) st.K -= log(mass);
     co = has_out ? sum_p * exp(shift) / S : S > 0 ? 0.0 : __builtin_nan("");  // a row of -inf has no distribution
   }
   if (!r.any) kd = 0;
@@ -896,7 +897,7 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, co
   if (h > 0) loss += h * (log(z1) - ((double)T::load(z[r.y]) - st.top));
   loss_rows[row] = (float)loss;
   st.co = (float)((w == 0 ? 0.0 : w * co) + (h > 0 && !two ? h * exp((double)st.ref - st.top) / z1 : 0.0));
-  st.ci = r.any && w != 0 ? (float)(w / S) : 0.f;
+  st.ci = r.any && w != 0 ? (float)(w * mass / S) : 0.f;
   st.h1 = h > 0 ? (float)(h / z1) : 0.f;
   st.used = 1.f;
   reinterpret_cast<RowStats*>(a.stats)[row] = st;
@@ -1077,7 +1078,7 @@ __global__ __launch_bounds__(kT) void distill_bwd_k(DistillArgs a, int nseg, int
         times += cls_s[j + e] == cls ? 1.f : 0.f;
       }
     }
-    float d = ci == 0.f ? 0.f : q * (1.f - times + st.over) - more;
+    float d = q * (1.f - times) - more;
     if (ci == 0.f) v = T::load(z[cls]);
     if (a.hard > 0) d += h1 * exp2f((v - m) * c1) - (cls == y ? (float)a.hard : 0.f);
     dz[cls] = T::store(g * d);

@@ -174,9 +174,10 @@ def _distill_kd(z, tv, ti, tlse, temperature, used, counted):
         by_sum = (over.detach().abs() < 0.2) & (q_out.detach() != 0)
         rest = torch.where(has, 1 - sum_p, 0.0)
         r = torch.where(has, rest, 1.0)
-        # log q_out, also where it is too small for a number
-        out = torch.where(live & ~named, dz / temperature, -math.inf)
-        log_q = torch.logsumexp(torch.where(has[:, None], out, 0.0), 1) - whole - part
+        # log q_out, also where it is too small for a number: from the maximum outside
+        out = torch.where(has[:, None], torch.where(live & ~named, dz, -math.inf), 0.0)
+        most = out.detach().amax(1, keepdim=True)
+        log_q = torch.logsumexp((out - most) / temperature, 1) + most[:, 0] / temperature - whole - part
         gain = torch.where(by_sum, q_out * _gain(torch.log1p(torch.where(by_sum, over, 0.0))),
                            r * (r.log() - log_q) - r + q_out)
         rest = torch.where(has, gain, (sum_p - 1) + q_out)

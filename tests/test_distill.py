@@ -551,6 +551,41 @@ def test_distill_loss_rows_of_one_value(dev, dtype, T):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1.0, 8.0, 50.0, 1e6])
+def test_distill_loss_little_left(dev, dtype, T):
+    """Rows of which the student leaves little: only classes at the type's lowest value outside the named
+    ones (they share the rest evenly), one class alone (its gradient is 0), a few, all of them named, and a
+    teacher whose normaliser counts the masked classes too."""
+    V, k = 30, 6
+    g = torch.Generator().manual_seed(5)
+    teacher = torch.randn(3, V, generator=g).to(dtype)
+    z = (teacher.float() + torch.randn(3, V, generator=g)).to(dtype)
+    tv, ti = (t[:, :k].contiguous() for t in torch.sort(teacher, dim=1, descending=True))
+    lse = torch.logsumexp(teacher.double() / T, 1).float()
+    out = torch.ones(3, V, dtype=torch.bool).scatter_(1, ti, False)
+    z[0, out[0]] = torch.finfo(dtype).min
+    z[1, torch.arange(V) != ti[1, 2]] = -INF
+    z[2, out[2]] = -INF
+    ti[1, [0, 1, 3, 4, 5]] = -1  # what the student masks is not named: its KL would be infinite
+    leaf = z.to(dev, copy=True).requires_grad_()
+    loss = ops.distill_loss(leaf, tv.to(dev), ti.to(dev), None, lse.to(dev), T, 0.0, "none")
+    grad, = torch.autograd.grad(loss.sum(), leaf)
+    fi = torch.finfo(dtype)
+    for r in range(3):
+        want, wg, q, _ = oracle_decimal(z[r].tolist(), tv[r].tolist(), ti[r].tolist(), None, lse[r].item(), T, 0.0)
+        if r and abs(want) < 3.4e38:
+            assert abs(loss[r].item() - want) <= T * T * es(V) + 2 * E * abs(want)
+        wg, q = torch.tensor(wg, dtype=torch.float64), torch.tensor(q, dtype=torch.float64)
+        # up to T = 8 the sums are fp32; above, a class's gradient is right to some steps of its own and
+        # T q 2^-50 (sizes of lse and of d)
+        tg = 32 * E * wg.abs() + T * q * (es(V) if T <= 8 else 2.0**-44)
+        tg = tg + fi.eps / 2 * 1.01 * (wg.abs() + tg) + fi.smallest_normal * fi.eps + 2.0**-126 * 2 * T
+        ok = (grad[r].cpu().double() - wg).abs() <= tg
+        assert bool((ok | (wg.abs() > fi.max)).all()), (r, grad[r].tolist(), wg.tolist())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_distill_loss_nothing(dev):
     """No rows; no row that counts; a left-out row whose logits and teacher hold NaN."""
     z, tv, ti, y, lse = make(4, 30, 3, torch.float32, 10)
