@@ -75,7 +75,7 @@ class DistributedDataParallel(nn.Module):
         self.flat_buffers = flatten_buffers(module, self.device) if broadcast_buffers else None
         self.flat_bytes = flatten_integer_buffers(module, self.device) if broadcast_buffers else None
         self.broadcast_buffers = broadcast_buffers and not (self.flat_buffers is None and self.flat_bytes is None)
-        self._counters = integer_counters(module) if broadcast_buffers else []
+        self._counters = integer_counters(module, self.device) if broadcast_buffers else []
         numels = [p.numel() for p in self.flat.params]
         self.buckets, self.param_bucket = assign_buckets(numels, self.flat.offsets, self.flat.numel, bucket_cap_mb,
                                                          first_bucket_cap_mb)

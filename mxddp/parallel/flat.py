@@ -87,15 +87,20 @@ def flatten_buffers(module: nn.Module, device: torch.device | None = None):
     return flat
 
 
-def flatten_integer_buffers(module: nn.Module, device: torch.device | None = None):
+def _integers(module: nn.Module, device: torch.device) -> list[torch.Tensor]:
+    """Integer buffers on the model's device; those that are kept elsewhere are the model's own affair."""
+    return [b for b in module.buffers()
+            if b.device == device and not b.is_floating_point() and not b.is_complex()]
+
+
+def flatten_integer_buffers(module: nn.Module, device: torch.device):
     """Re-home integer buffers (the weight of an 8-bit layer) into one flat byte tensor, broadcast
     together with the floating-point ones: such a weight means nothing without its own scales.
     Counters (num_batches_tracked, no dimensions) stay where they are: they are broadcast at wrap
     time only (``integer_counters``), every rank counting the same steps from there."""
-    bufs = [b for b in module.buffers() if not b.is_floating_point() and not b.is_complex() and b.dim() > 0]
+    bufs = [b for b in _integers(module, device) if b.dim() > 0]
     if not bufs:
         return None
-    device = device or bufs[0].device
     size = lambda b: _al(b.numel() * b.element_size() // 4 + 1) * 4  # noqa: E731 - bytes, 64-byte starts
     flat = torch.zeros(sum(size(b) for b in bufs), dtype=torch.uint8, device=device)
     off = 0
@@ -108,5 +113,5 @@ def flatten_integer_buffers(module: nn.Module, device: torch.device | None = Non
     return flat
 
 
-def integer_counters(module: nn.Module) -> list[torch.Tensor]:
-    return [b for b in module.buffers() if not b.is_floating_point() and not b.is_complex() and b.dim() == 0]
+def integer_counters(module: nn.Module, device: torch.device) -> list[torch.Tensor]:
+    return [b for b in _integers(module, device) if b.dim() == 0]

@@ -30,6 +30,9 @@ def _model(seed):
             self.head = Linear(16, 5)
             self.register_buffer("kinds", torch.tensor([[seed, 2], [3, 4]], dtype=torch.int32))
             self.register_buffer("flags", torch.tensor([seed > 1, True, False]))
+            self.register_buffer("empty", torch.zeros(0, 3, dtype=torch.int64))
+            self.register_buffer("elsewhere", torch.zeros(3, dtype=torch.int32, device="meta"), persistent=False)
+            self.register_buffer("count_elsewhere", torch.zeros((), dtype=torch.int64, device="meta"), persistent=False)
             self.bn.num_batches_tracked.fill_(seed)
 
         def trunk(self, x):
@@ -55,7 +58,13 @@ def _worker(rank, ws, port, gpu, broadcast, q):
             comm.init_distributed(rank=rank, world_size=ws, use_gpu=False, init_method=f"tcp://127.0.0.1:{port}")
         dev = torch.device("cuda", 0) if gpu else torch.device("cpu")
         x = torch.randn(6, 20, generator=torch.Generator().manual_seed(3)).to(dev)
-        model = _model(1 + rank).to(dev)
+        model = _model(1 + rank)
+        meta = {n: b for n, b in model.named_buffers() if b.is_meta}
+        for n in meta:
+            delattr(model, n)
+        model.to(dev)
+        for n, b in meta.items():
+            model.register_buffer(n, b, persistent=False)
         ddp = DDP(model, broadcast_buffers=broadcast)
         out = []
 
