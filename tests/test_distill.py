@@ -854,6 +854,69 @@ def test_distill_graph(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V", [(520, 140001), (2, 140001)])
+def test_distill_loss_long_rows_high_temperature(cuda, dtype, N, V):
+    """Above T = 8: rows longer than the classes whose marks are in LDS at a time, in one block each and split
+    over blocks; each of the named classes holds a percent of the row, so one that is taken for the wrong
+    side shows.  Both passes repeat bit by bit."""
+    k, T = 40, 20.0
+    g = torch.Generator().manual_seed(V)
+    rows = [0, N - 1]
+    ti = torch.randint(V, (N, k), generator=g)
+    ti[rows, 0], ti[rows, 1] = V - 1, 65536
+    few = (2 * torch.randn(2, V, generator=g)).scatter_(1, ti[rows], 150.0).to(dtype)
+    tv = (torch.randn(N, k, generator=g) + 148).to(dtype)
+    lse = torch.full((N,), 12.0)
+    y = torch.full((N,), -100)
+    y[rows] = torch.tensor([3, V - 1])
+    z = torch.zeros(N, V, dtype=dtype, device=cuda)
+    z[rows] = few.to(cuda)
+    z.requires_grad_()
+    out = []
+    for _ in range(2):
+        loss = ops.distill_loss(z, tv.to(cuda), ti.to(cuda), y.to(cuda), lse.to(cuda), T, 0.5, "none")
+        out.append((loss.detach(), torch.autograd.grad(loss.sum(), z)[0][rows].cpu().double()))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+    want, _, grad, _, _ = oracle(few, tv[rows], ti[rows], y[rows], lse[rows], T, 0.5)
+    assert (want > 1).all()
+    # sums in 64 bits; the labels' in fp32: es(V) of its logarithm
+    assert bool(((out[0][0][rows].cpu().double() - want).abs() <= 4 * E * want + es(V)).all())
+    assert N == 2 or not out[0][0][1:-1].any()
+    tol = 64 * E * (grad.abs() + T / V) + es(V) * torch.softmax(few.double(), 1)
+    tol = tol + torch.finfo(dtype).eps / 2 * 1.01 * (grad.abs() + tol) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert bool(((out[0][1] - grad).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+def test_distill_graph_high_temperature(cuda):
+    """Loss and gradient above T = 8 captured, with rows that are split over blocks, and replayed with new
+    logits and eager calls in between."""
+    z, tv, ti, y, lse = make(3, 20000, 12, torch.float16, 18, 30.0)
+    tv, ti, y, lse = tv.to(cuda), ti.to(cuda), y.to(cuda), lse.to(cuda)
+
+    def step(leaf):
+        loss = ops.distill_loss(leaf, tv, ti, y, lse, 30.0, 0.5)
+        return loss.detach(), torch.autograd.grad(loss, leaf)[0]
+
+    leaf = z.to(cuda).requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(leaf)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(leaf)
+    for i in range(3):
+        with torch.no_grad():
+            leaf.copy_(z.to(cuda) * (1 + i))
+        graph.replay()
+        loss, grad = step(leaf)
+        assert torch.equal(out[0], loss) and torch.equal(out[1], grad), i
+
+
+@pytest.mark.gpu
 def test_distill_other_stream(cuda):
     z, tv, ti, y, lse = make(8, 5000, 9, torch.float32, 16)
     st = torch.cuda.Stream()
