@@ -584,8 +584,9 @@ __device__ __forceinline__ void load_entry(const DistillArgs& a, int64_t row, in
 // once a piece.  Backward: the same pieces, read again and written; the named classes and the label
 // are written over afterwards by their own threads.  The gradient is not written by the forward: that
 // would save a pass only where the loss's own gradient is 1, and cost one (870 us for 600) elsewhere.
-// 4096 x 131072 in bf16 with the teacher's normaliser: forward 184 us (5.8 TB/s), backward 418 us (5.1
-// TB/s); 1023 x 50001 in fp16: 32 to 39 us and 40 us (rows of no alignment; 32 and 37 with rows of 50048).
+// 4096 x 131072 in bf16 with the teacher's normaliser: forward 184 us (a plain read's rate), backward
+// 418 us (5.1 TB/s); 1023 x 50001 in fp16: 30 to 35 us and 40 to 47 us (rows of no alignment; 32 and 37 with
+// rows of 50048).
 //
 // T^2 KD is of the logits' size at any T, so KD is of 1 / T^2, and what it is made of must not be
 // rounded at 1.  A row's sum of exponentials is held as S = n + e.  Up to T = kNearT n = 0 and e is a sum of

@@ -2,8 +2,9 @@
 
 ``top_logits`` keeps what a teacher's answer needs: its k largest logits, their classes, and the
 logarithm of the whole sum of exponentials.  ``distill_loss`` is the student's loss against them,
-with the labels' cross-entropy mixed in where it is asked for; its forward reads the logits once, its
-backward reads them once more and writes their gradient.
+with the labels' cross-entropy mixed in where it is asked for; its forward reads the logits once (twice
+above a temperature of 8, where it adds up in 64 bits), its backward reads them once more and writes
+their gradient.
 """
 from __future__ import annotations
 
